@@ -23,6 +23,9 @@ SOURCES = [
     "reduce.hip",
     "softmax.hip",
     "layernorm.hip",
+    "layernorm_bwd.hip",
+    "gated.hip",
+    "dropout.hip",
     "index.hip",
     "gemm.hip",
     "gemm_x16.hip",
@@ -47,7 +50,7 @@ def _fresh(src: str, obj: Path) -> bool:
     """True when `obj` is newer than its source and every header beside it."""
     if not obj.exists():
         return False
-    deps = [CSRC / src, *CSRC.glob("*.h"), PKG_DIR.parent / "include" / "mi355_aten.h", Path(__file__)]
+    deps = [CSRC / src, *CSRC.glob("*.h"), *(PKG_DIR.parent / "include").glob("*.h"), Path(__file__)]
     return obj.stat().st_mtime > max(d.stat().st_mtime for d in deps)
 
 

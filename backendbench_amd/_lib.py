@@ -1,4 +1,4 @@
-"""ctypes binding of libmi355_aten.so (declared in include/mi355_aten.h).
+"""ctypes binding of libmi355_aten.so (declared in include/mi355_aten.h and include/mi355_train.h).
 
 This is the only place that touches the C ABI.  There is no fallback: if the library has
 not been built, or its ABI version differs, loading raises and every operator wrapper
@@ -34,6 +34,8 @@ DTYPE = {
 ADD, MUL, MAXIMUM, MINIMUM = 0, 1, 2, 3
 RELU, CLAMP = 0, 1
 SUM, MEAN, AMAX, ARGMAX = 0, 1, 2, 3
+# mi355_activation
+SILU, GELU, GELU_TANH = 0, 1, 2
 
 
 class TensorDesc(ctypes.Structure):
@@ -106,6 +108,22 @@ SIGNATURES = {
     "mi355_gather": (c_int, [_P, c_int, _P, _P, c_void_p, c_void_p]),
 }
 
+# The training operators; mirrors include/mi355_train.h one to one.
+TRAIN_SIGNATURES = {
+    "mi355_layer_norm_backward_workspace_bytes": (c_int64, [c_int64, c_int64, c_int]),
+    "mi355_layer_norm_backward": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+         c_void_p, c_int64, c_void_p],
+    ),
+    "mi355_gated_act": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p]),
+    "mi355_gated_act_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p]),
+    "mi355_dropout_add": (
+        c_int,
+        [c_void_p, c_void_p, c_int, c_double, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p],
+    ),
+}
+
 _lib = None
 
 
@@ -120,7 +138,7 @@ def load():
             "(python -m backendbench_amd._build); there is no fallback path"
         )
     lib = ctypes.CDLL(str(LIB_PATH))
-    for name, (restype, argtypes) in SIGNATURES.items():
+    for name, (restype, argtypes) in {**SIGNATURES, **TRAIN_SIGNATURES}.items():
         fn = getattr(lib, name)  # AttributeError if a declared symbol is not exported
         fn.restype = restype
         fn.argtypes = argtypes

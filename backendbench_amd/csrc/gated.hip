@@ -1,0 +1,128 @@
+// The gated projection of a feed-forward block: h = act(x Wg^T) * (x Wu^T), W = [Wg; Wu] of 2F rows, and the
+// elementwise part of its backward pass.
+#include "gated.h"
+#include "elementwise.h"
+
+namespace mi355 {
+
+// Columns f .. f + V - 1 of one row per work item.  P: type of pre as read.
+template <typename T, typename P, int ACT, int V, bool SAVE>
+__global__ __launch_bounds__(256) void gated_act_kernel(const P* __restrict__ pre, T* __restrict__ h, T* __restrict__ pre_out,
+                                                       int64_t items, int64_t per_row, int64_t F) {
+  using A = typename OpMath<T>::type;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = items < (int64_t(1) << 32) ? (uint32_t)i / (uint32_t)per_row : i / per_row;
+    const int64_t f = (i - m * per_row) * V;
+    const VecN<P, V> g = ld_nt<P, V>(pre + m * 2 * F + f), u = ld_nt<P, V>(pre + m * 2 * F + F + f);
+    VecN<T, V> r, sg, su;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const A ga = static_cast<A>(g.v[j]), ua = static_cast<A>(u.v[j]);
+      r.v[j] = static_cast<T>(ga * gate_q<ACT, A>(ga) * ua);
+      if constexpr (SAVE) {
+        sg.v[j] = static_cast<T>(ga);
+        su.v[j] = static_cast<T>(ua);
+      }
+    }
+    st<T, V>(h + m * F + f, r);
+    if constexpr (SAVE) {
+      st<T, V>(pre_out + m * 2 * F + f, sg);
+      st<T, V>(pre_out + m * 2 * F + F + f, su);
+    }
+  }
+}
+
+template <typename T, int ACT, int V>
+__global__ __launch_bounds__(256) void gated_act_backward_kernel(const T* __restrict__ dh, const T* __restrict__ pre,
+                                                                T* __restrict__ dpre, int64_t items, int64_t per_row, int64_t F) {
+  using A = typename OpMath<T>::type;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = items < (int64_t(1) << 32) ? (uint32_t)i / (uint32_t)per_row : i / per_row;
+    const int64_t f = (i - m * per_row) * V;
+    const VecN<T, V> g = ld_nt<T, V>(pre + m * 2 * F + f), u = ld_nt<T, V>(pre + m * 2 * F + F + f), d = ld_nt<T, V>(dh + m * F + f);
+    VecN<T, V> dg, du;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const A ga = static_cast<A>(g.v[j]), ua = static_cast<A>(u.v[j]), da = static_cast<A>(d.v[j]);
+      const A q = gate_q<ACT, A>(ga);
+      dg.v[j] = static_cast<T>(da * ua * gate_grad<ACT, A>(ga, q));
+      du.v[j] = static_cast<T>(da * (ga * q));
+    }
+    st<T, V>(dpre + m * 2 * F + f, dg);
+    st<T, V>(dpre + m * 2 * F + F + f, du);
+  }
+}
+
+// body(ACT) with an integral constant.
+template <typename Body> static int dispatch_act(int act, const char* name, Body body) {
+  switch (act) {
+    case MI355_SILU: body(std::integral_constant<int, MI355_SILU>()); return MI355_OK;
+    case MI355_GELU: body(std::integral_constant<int, MI355_GELU>()); return MI355_OK;
+    case MI355_GELU_TANH: body(std::integral_constant<int, MI355_GELU_TANH>()); return MI355_OK;
+    default: return set_error(MI355_ERR_INVALID, "%s: unknown activation %d", name, act);
+  }
+}
+
+template <typename T, typename P>
+static int run_gated_act(const void* pre, void* h, void* pre_out, int64_t M, int64_t F, int act, hipStream_t st) {
+  constexpr int V = 16 / sizeof(P);  // whole 16-byte reads
+  const bool vec = F % V == 0 && aligned16(pre) && aligned16(h) && aligned16(pre_out);
+  const int rc = dispatch_act(act, "mi355_gated_act", [&](auto a) {
+    constexpr int ACT = decltype(a)::value;
+    auto go = [&](auto v, auto save) {
+      constexpr int VV = decltype(v)::value;
+      const int64_t items = M * (F / VV);
+      hipLaunchKernelGGL((gated_act_kernel<T, P, ACT, VV, decltype(save)::value>), dim3((unsigned)grid_for(items, 256, 1 << 20)), dim3(256), 0, st,
+                         static_cast<const P*>(pre), static_cast<T*>(h), static_cast<T*>(pre_out), items, F / VV, F);
+    };
+    using std::integral_constant;
+    if (pre_out != nullptr) vec ? go(integral_constant<int, V>(), std::true_type()) : go(integral_constant<int, 1>(), std::true_type());
+    else vec ? go(integral_constant<int, V>(), std::false_type()) : go(integral_constant<int, 1>(), std::false_type());
+  });
+  return rc != MI355_OK ? rc : check_launch("mi355_gated_act");
+}
+
+template <typename T>
+static int run_gated_act_backward(const void* dh, const void* pre, void* dpre, int64_t M, int64_t F, int act, hipStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = F % V == 0 && aligned16(pre) && aligned16(dh) && aligned16(dpre);
+  const int rc = dispatch_act(act, "mi355_gated_act_backward", [&](auto a) {
+    constexpr int ACT = decltype(a)::value;
+    auto go = [&](auto v) {
+      constexpr int VV = decltype(v)::value;
+      const int64_t items = M * (F / VV);
+      hipLaunchKernelGGL((gated_act_backward_kernel<T, ACT, VV>), dim3((unsigned)grid_for(items, 256, 1 << 20)), dim3(256), 0, st,
+                         static_cast<const T*>(dh), static_cast<const T*>(pre), static_cast<T*>(dpre), items, F / VV, F);
+    };
+    vec ? go(std::integral_constant<int, V>()) : go(std::integral_constant<int, 1>());
+  });
+  return rc != MI355_OK ? rc : check_launch("mi355_gated_act_backward");
+}
+
+}  // namespace mi355
+
+using namespace mi355;
+
+extern "C" int mi355_gated_act(const void* pre, int pre_dtype, void* h, void* pre_out, int dtype, int64_t M, int64_t F, int act,
+                               void* stream) {
+  MI355_REQUIRE(M >= 0 && F >= 0, "mi355_gated_act: negative extent");
+  MI355_REQUIRE(act >= MI355_SILU && act <= MI355_GELU_TANH, "mi355_gated_act: unknown activation %d", act);
+  if (M == 0 || F == 0) return MI355_OK;
+  MI355_REQUIRE(pre != nullptr && h != nullptr, "mi355_gated_act: NULL data pointer");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (pre_dtype == MI355_F32 && dtype == MI355_F16) return run_gated_act<f16_t, float>(pre, h, pre_out, M, F, act, st);
+  if (pre_dtype == MI355_F32 && dtype == MI355_BF16) return run_gated_act<bf16_t, float>(pre, h, pre_out, M, F, act, st);
+  if (pre_dtype != dtype)
+    return set_error(MI355_ERR_UNSUPPORTED, "mi355_gated_act: no kernel for %s from %s", dtype_name(dtype), dtype_name(pre_dtype));
+  MI355_DISPATCH_FLOAT(dtype, "mi355_gated_act", return run_gated_act<T, T>(pre, h, pre_out, M, F, act, st));
+}
+
+extern "C" int mi355_gated_act_backward(const void* dh, const void* pre, void* dpre, int dtype, int64_t M, int64_t F, int act,
+                                        void* stream) {
+  MI355_REQUIRE(M >= 0 && F >= 0, "mi355_gated_act_backward: negative extent");
+  MI355_REQUIRE(act >= MI355_SILU && act <= MI355_GELU_TANH, "mi355_gated_act_backward: unknown activation %d", act);
+  if (M == 0 || F == 0) return MI355_OK;
+  MI355_REQUIRE(dh != nullptr && pre != nullptr && dpre != nullptr, "mi355_gated_act_backward: NULL data pointer");
+  MI355_DISPATCH_FLOAT(dtype, "mi355_gated_act_backward",
+                       return run_gated_act_backward<T>(dh, pre, dpre, M, F, act, static_cast<hipStream_t>(stream)));
+}

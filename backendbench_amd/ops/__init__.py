@@ -4,7 +4,8 @@ SLOTS maps the directory-backend folder name (BackendBench/utils.py:289-308 nami
 callable that fills `<folder>_kernel_impl`.  CORE_SLOTS are the 19 overloads of the core
 operator set; VARIANT_SLOTS are their in-place / out= / sibling overloads
 (BackendBench/scripts/op_map.py lists them on the same `canonical:` lines), served by the
-same kernels.
+same kernels.  TRAINING_SLOTS are the overloads of a training step, kept in a folder tree of their own; the operators
+beside them that ATen has no overload for (gated_linear, dropout_add and their backward passes) are called from here.
 """
 
 from ._common import check_index_errors
@@ -15,6 +16,8 @@ from .index import embedding, gather, index_select
 from .matmul import addmm, addmm_dtype, mm, mm_dtype
 from .reduce import (amax, argmax, log_softmax, mean_default, mean_dim, native_layer_norm, softmax, sum_default,
                      sum_dim)
+from .training import (dropout_add, dropout_add_backward, dropout_counters, gated_linear, gated_linear_backward,
+                       native_layer_norm_backward, native_layer_norm_backward_out)
 
 CORE_SLOTS = {
     "add__Tensor": add,
@@ -95,4 +98,11 @@ VARIANT_SLOTS = {
 
 SLOTS = {**CORE_SLOTS, **VARIANT_SLOTS}
 
-__all__ = ["SLOTS", "CORE_SLOTS", "VARIANT_SLOTS", "check_index_errors"]
+# Folders of the training tree (create_kernel_directory --training): enable() takes it after, or instead of, the other one.
+TRAINING_SLOTS = {
+    "native_layer_norm_backward__default": native_layer_norm_backward,
+    "native_layer_norm_backward__out": native_layer_norm_backward_out,
+}
+
+__all__ = ["SLOTS", "CORE_SLOTS", "VARIANT_SLOTS", "TRAINING_SLOTS", "check_index_errors", "dropout_add", "dropout_add_backward",
+           "dropout_counters", "gated_linear", "gated_linear_backward", "native_layer_norm_backward"]

@@ -65,7 +65,28 @@ def device_managed(fn):
             return out
         if isinstance(out, torch.Tensor):
             return out.to(home)
-        return tuple(o.to(home) for o in out)
+        return tuple(o if o is None else o.to(home) for o in out)
+
+    return wrapper
+
+
+def on_device_of_arguments(fn):
+    """Run `fn` with the GPU of its tensor arguments current, so that its launches go to that GPU's current stream;
+    tensors on more than one GPU are refused.  Goes under device_managed, which brings every tensor to a GPU."""
+
+    @functools.wraps(fn)
+    def wrapper(*args, **kwargs):
+        device = None
+        for a in (*args, *kwargs.values()):
+            if isinstance(a, torch.Tensor):
+                if device is None:
+                    device = a.device
+                elif a.device != device:
+                    raise RuntimeError(f"Expected all tensors to be on the same device, but found at least two devices, {device} and {a.device}!")
+        if device is None or device.index == _current_device():
+            return fn(*args, **kwargs)
+        with torch.cuda.device(device):
+            return fn(*args, **kwargs)
 
     return wrapper
 

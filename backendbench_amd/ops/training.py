@@ -1,0 +1,252 @@
+"""Operators of a training step: layer norm's backward pass, the gated linear projection of a feed-forward block with
+its backward pass, and dropout from a counter-based generator with the residual add.
+
+Like the ATen overloads beside them these are kernels, not autograd nodes: they return plain results, and a gradient is
+a call of the operator that computes it.  Arguments are checked before anything touches the GPU.
+"""
+
+import torch
+
+from .. import _lib
+from ._common import (cast, copy_into, dense, device_managed, launch, new_dense, new_result, on_device_of_arguments, prod)
+from .elementwise import _store_result as store_result
+from .elementwise import tuple_out_variant
+from .matmul import _gemm, _gemm_f32out
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16, torch.float64)
+_HALF = (torch.bfloat16, torch.float16)
+
+
+def _need_float(t, what):
+    if t.dtype not in _FLOATS:
+        raise NotImplementedError(f"mi355 backend: {what} on {t.dtype} is not supported")
+
+
+# ---- layer norm, backward ------------------------------------------------------------------------------------------
+def native_layer_norm_backward(grad_out, input, normalized_shape, mean, rstd, weight, bias, output_mask):
+    """aten.native_layer_norm_backward.default -> (grad_input, grad_weight, grad_bias), None where output_mask is False.
+
+    mean and rstd are what native_layer_norm returned; grad_weight and grad_bias have the dtype of weight and bias."""
+    k = len(normalized_shape)
+    if k == 0 or list(input.shape[input.dim() - k :]) != list(normalized_shape):
+        raise RuntimeError(
+            f"Given normalized_shape={list(normalized_shape)}, expected input with shape "
+            f"[*, {', '.join(str(s) for s in normalized_shape)}], but got input of size{list(input.shape)}")
+    _need_float(input, "layer norm")
+    if grad_out.shape != input.shape:
+        raise RuntimeError(f"Expected grad_out of the input's shape {list(input.shape)}, but got {list(grad_out.shape)}")
+    if grad_out.dtype != input.dtype:
+        raise RuntimeError(f"Expected grad_out of the input's dtype {input.dtype}, but got {grad_out.dtype}")
+    M = prod(input.shape[: input.dim() - k])
+    for name, s in (("mean", mean), ("rstd", rstd)):
+        if s.numel() != M:
+            raise RuntimeError(f"Expected {name} to hold {M} values, one per row, but got {s.numel()}")
+        _need_float(s, f"layer norm statistics ({name})")
+    for i, (name, p) in enumerate((("weight", weight), ("bias", bias))):
+        if p is None:
+            if output_mask[i + 1]:
+                raise RuntimeError(f"the gradient of {name} was asked for, but {name} is None")
+        elif list(p.shape) != list(normalized_shape):
+            raise RuntimeError(f"Expected {name} to be of same shape as normalized_shape, but got {name} of shape "
+                               f"{list(p.shape)} and normalized_shape = {list(normalized_shape)}")
+        else:
+            _need_float(p, f"layer norm {name}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise RuntimeError("weight and bias must have the same dtype")
+    return _layer_norm_backward(grad_out, input, list(normalized_shape), mean, rstd, weight, bias, [bool(v) for v in output_mask])
+
+
+@device_managed
+@on_device_of_arguments
+def _layer_norm_backward(grad_out, input, normalized_shape, mean, rstd, weight, bias, mask):
+    k = len(normalized_shape)
+    M, N = prod(input.shape[: input.dim() - k]), prod(normalized_shape)
+    w_given = weight.dtype if weight is not None else bias.dtype if bias is not None else input.dtype
+    dx = new_result(input.shape, input.dtype, input.device) if mask[0] else None
+    grads = [new_result(normalized_shape, w_given, input.device) if m else None for m in mask[1:]]
+    if M == 0 or N == 0 or not any(mask):
+        for g in grads:
+            if g is not None:
+                g.zero_()
+        return dx, grads[0], grads[1]
+    # the kernels take parameters of the rows' dtype, or fp32 beside bf16 / f16 rows
+    w_dtype = w_given if w_given == input.dtype or (w_given == torch.float32 and input.dtype in _HALF) else input.dtype
+    if w_dtype != w_given and input.dtype in _HALF:
+        w_dtype = torch.float32  # (fp64 or the other half type: through fp32, not through the narrower type)
+    stat_dtype = torch.float64 if input.dtype == torch.float64 else torch.float32
+    x, dy = dense(input), dense(grad_out)
+    mu, rs = dense(cast(mean, stat_dtype)), dense(cast(rstd, stat_dtype))
+    w = dense(cast(weight, w_dtype)) if weight is not None else None
+    outs = [g if g is None or g.dtype == w_dtype else new_dense(g.shape, w_dtype, g.device) for g in grads]
+    code = _lib.dtype_code(input.dtype)
+    ws_bytes = _lib.load().mi355_layer_norm_backward_workspace_bytes(M, N, code)
+    ws = new_dense((ws_bytes,), torch.uint8, input.device)
+
+    def ptr(t):
+        return t.data_ptr() if t is not None else None
+
+    launch("mi355_layer_norm_backward", dy.data_ptr(), x.data_ptr(), code, mu.data_ptr(), rs.data_ptr(), ptr(w),
+           _lib.dtype_code(w_dtype), ptr(dx), ptr(outs[0]), ptr(outs[1]), M, N, ws.data_ptr(), ws_bytes)
+    for g, o in zip(grads, outs):
+        if g is not o:
+            copy_into(g, o)
+    return dx, grads[0], grads[1]
+
+
+_out_all = tuple_out_variant(native_layer_norm_backward, 3)
+
+
+def native_layer_norm_backward_out(grad_out, input, normalized_shape, mean, rstd, weight, bias, output_mask, *, out0, out1, out2):
+    """aten.native_layer_norm_backward.out; an out tensor whose output_mask entry is False is left as it is."""
+    args = (grad_out, input, normalized_shape, mean, rstd, weight, bias, output_mask)
+    if all(output_mask):
+        return _out_all(*args, out0=out0, out1=out1, out2=out2)
+    results = native_layer_norm_backward(*args)
+    return tuple(o if r is None else store_result(o, r) for o, r in zip((out0, out1, out2), results))
+
+
+# ---- gated linear projection ---------------------------------------------------------------------------------------
+_ACTIVATIONS = {"silu": _lib.SILU, "gelu": _lib.GELU, "gelu_tanh": _lib.GELU_TANH}
+
+
+def _check_gated(input, weight, activation):
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+    _need_float(input, "gated_linear")
+    if weight.dtype != input.dtype:
+        raise RuntimeError(f"expected input and weight to have the same dtype, but got: {input.dtype} != {weight.dtype}")
+    if weight.dim() != 2 or weight.shape[0] % 2:
+        raise RuntimeError(f"weight must be [2 * features, in_features] (gate rows, then up rows), got {list(weight.shape)}")
+    if input.dim() == 0 or input.shape[-1] != weight.shape[1]:
+        raise RuntimeError(f"input {list(input.shape)} and weight {list(weight.shape)} cannot be multiplied: the last dimension of "
+                           "input must be weight's second")
+
+
+def gated_linear(input, weight, activation="silu", save_pre=False):
+    """act(input @ weight[:F].T) * (input @ weight[F:].T) over the last dimension of input; weight is [2F, K].
+
+    activation: "silu", "gelu" (by the error function) or "gelu_tanh".  Products are accumulated in fp32 (fp64 for
+    fp64) and not rounded before the activation.  save_pre: also return the pre-activations [..., 2F] in the input's
+    dtype, which gated_linear_backward takes; the one rounding between the two passes."""
+    _check_gated(input, weight, activation)
+    return _gated_linear(input, weight, activation, bool(save_pre))
+
+
+@device_managed
+@on_device_of_arguments
+def _gated_linear(input, weight, activation, save_pre):
+    lead, K = list(input.shape[:-1]), input.shape[-1]
+    M, F = prod(lead), weight.shape[0] // 2
+    dtype, device = input.dtype, input.device
+    if M == 0 or F == 0 or K == 0:  # (no terms: pre = 0 and act(0) = 0)
+        h = torch.zeros(lead + [F], dtype=dtype, device=device)
+        return (h, torch.zeros(lead + [2 * F], dtype=dtype, device=device)) if save_pre else h
+    h = new_dense(lead + [F], dtype, device)
+    pre = new_dense(lead + [2 * F], dtype, device) if save_pre else None
+    x = dense(input).view(M, K)
+    if dtype in _HALF:
+        wide = _gemm_f32out(x, weight.t(), None, 1.0, 0.0)
+        saved = pre
+    else:
+        wide = _gemm(x, weight.t(), None, 1.0, 0.0)
+        saved = None
+        if save_pre:
+            pre = wide.view(lead + [2 * F])
+    launch("mi355_gated_act", wide.data_ptr(), _lib.dtype_code(wide.dtype), h.data_ptr(),
+           saved.data_ptr() if saved is not None else None, _lib.dtype_code(dtype), M, F, _ACTIVATIONS[activation])
+    return (h, pre) if save_pre else h
+
+
+def gated_linear_backward(grad_out, input, weight, pre, activation="silu", output_mask=(True, True)):
+    """Gradients of gated_linear -> (grad_input, grad_weight), None where output_mask is False.
+
+    pre: the pre-activations gated_linear(..., save_pre=True) returned.  The gradient of pre is computed in fp32 and
+    rounded once to the input's dtype: it is the operand of the two matrix products, which accumulate in fp32."""
+    _check_gated(input, weight, activation)
+    F = weight.shape[0] // 2
+    lead = list(input.shape[:-1])
+    for name, t, last in (("grad_out", grad_out, F), ("pre", pre, 2 * F)):
+        if list(t.shape) != lead + [last]:
+            raise RuntimeError(f"Expected {name} of shape {lead + [last]}, but got {list(t.shape)}")
+        if t.dtype != input.dtype:
+            raise RuntimeError(f"Expected {name} of the input's dtype {input.dtype}, but got {t.dtype}")
+    if len(output_mask) != 2:
+        raise RuntimeError(f"output_mask must have 2 entries, got {len(output_mask)}")
+    return _gated_linear_backward(grad_out, input, weight, pre, activation, [bool(v) for v in output_mask])
+
+
+@device_managed
+@on_device_of_arguments
+def _gated_linear_backward(grad_out, input, weight, pre, activation, mask):
+    K, F = weight.shape[1], weight.shape[0] // 2
+    M = prod(input.shape[:-1])
+    dtype, device = input.dtype, input.device
+    if M == 0 or F == 0 or K == 0 or not any(mask):
+        return (torch.zeros_like(input) if mask[0] else None), (torch.zeros_like(weight) if mask[1] else None)
+    dh, p, x = dense(grad_out), dense(pre), dense(input).view(M, K)
+    dpre = new_dense((M, 2 * F), dtype, device)
+    launch("mi355_gated_act_backward", dh.data_ptr(), p.data_ptr(), dpre.data_ptr(), _lib.dtype_code(dtype), M, F,
+           _ACTIVATIONS[activation])
+    dx = _gemm(dpre, weight, None, 1.0, 0.0).view(input.shape) if mask[0] else None
+    dw = _gemm(dpre.t(), x, None, 1.0, 0.0) if mask[1] else None
+    return dx, dw
+
+
+# ---- dropout with a residual ---------------------------------------------------------------------------------------
+def dropout_counters(numel):
+    """Counters a dropout_add over `numel` elements uses up: the next call's offset is this one's plus that."""
+    return (numel + 7) // 8
+
+
+def _check_dropout(x, p, rng):
+    _need_float(x, "dropout")
+    if not 0.0 <= p <= 1.0:
+        raise RuntimeError(f"dropout probability has to be between 0 and 1, but got {p}")
+    if isinstance(rng, torch.Tensor):
+        if rng.dtype != torch.int64 or list(rng.shape) != [2]:
+            raise RuntimeError(f"rng must hold two int64 values, (seed, offset), got {rng.dtype} {list(rng.shape)}")
+    elif len(rng) != 2:
+        raise RuntimeError(f"rng must hold two values, (seed, offset), got {len(rng)}")
+
+
+def dropout_add(input, residual, p, rng):
+    """residual + dropout(input, p) (residual None: dropout(input, p)); the mask is never stored.
+
+    rng: (seed, offset), two Python integers or an int64 tensor of two.  An int64 tensor on the GPU is read by the
+    kernel, so a captured graph draws anew once the program has advanced it.  Element i of input (in row-major order,
+    whatever its strides) takes the i % 8-th 16 bits of Philox-4x32-10 at counter offset + i // 8 under key seed and is
+    dropped when they are below t = round(p * 65536); what is kept is scaled by 65536 / (65536 - t), which makes the
+    expectation exact for the p that 16 bits can hold.  Advance the offset by dropout_counters(input.numel())."""
+    _check_dropout(input, p, rng)
+    if residual is not None and (residual.shape != input.shape or residual.dtype != input.dtype):
+        raise RuntimeError(f"Expected residual of the input's shape and dtype, {list(input.shape)} {input.dtype}, but got "
+                           f"{list(residual.shape)} {residual.dtype}")
+    return _dropout_add(input, residual, float(p), rng)
+
+
+def dropout_add_backward(grad_out, p, rng):
+    """Gradient of dropout_add with respect to its input, from the same p and rng (the residual's is grad_out itself)."""
+    _check_dropout(grad_out, p, rng)
+    return _dropout_add(grad_out, None, float(p), rng)
+
+
+def _int64(v):
+    return (int(v) + 2 ** 63) % 2 ** 64 - 2 ** 63
+
+
+@device_managed
+@on_device_of_arguments
+def _dropout_add(input, residual, p, rng):
+    out = new_dense(input.shape, input.dtype, input.device)
+    if input.numel() == 0:
+        return out
+    x = dense(input)
+    res = dense(residual) if residual is not None else None
+    words, seed, offset = None, 0, 0
+    if isinstance(rng, torch.Tensor):
+        words = dense(rng)
+    else:
+        seed, offset = (_int64(v) for v in rng)
+    launch("mi355_dropout_add", x.data_ptr(), res.data_ptr() if res is not None else None, _lib.dtype_code(x.dtype), p,
+           words.data_ptr() if words is not None else None, seed, offset, out.data_ptr(), x.numel())
+    return out

@@ -1,0 +1,63 @@
+/*
+ * mi355_train.h - C ABI of the training operators in libmi355_aten.so: layer norm's backward pass, the gated
+ * linear projection of a feed-forward block with its backward pass, and dropout from a counter-based generator
+ * with the residual add.  Conventions, status codes and dtypes are those of mi355_aten.h: device pointers, extents
+ * and strides in elements, kernels only enqueued on `stream`, nothing launched on error, 0 on success.
+ */
+#ifndef MI355_TRAIN_H
+#define MI355_TRAIN_H
+
+#include "mi355_aten.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* ---- layer norm, backward ---------------------------------------------------------- */
+
+/* For M dense rows of N elements, with xhat = (x - mean) * rstd and g = dy * weight (weight NULL: g = dy):
+ *   dx = rstd * (g - mean_N(g) - xhat * mean_N(g * xhat)),  dweight = sum_M dy * xhat,  dbias = sum_M dy.
+ * Any of dx, dweight, dbias may be NULL (not wanted).  dy, x, dx: `dtype` (f32, f16, bf16, f64); weight, dweight,
+ * dbias: `w_dtype` (dtype, or f32 for f16 / bf16 rows); mean, rstd: M values each, f32 (f64 for f64 rows).  Sums are
+ * held in fp32 (fp64 for f64 rows) and added in a fixed order: the same call gives the same bits.
+ * The workspace (contents undefined before and after) must hold mi355_layer_norm_backward_workspace_bytes() bytes,
+ * 16-byte aligned; a call with less is refused.
+ * Slot: native_layer_norm_backward__default. */
+int64_t mi355_layer_norm_backward_workspace_bytes(int64_t M, int64_t N, int dtype);
+int mi355_layer_norm_backward(const void* dy, const void* x, int dtype, const void* mean, const void* rstd,
+                              const void* weight, int w_dtype, void* dx, void* dweight, void* dbias, int64_t M, int64_t N,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- gated linear projection ------------------------------------------------------- */
+
+typedef enum mi355_activation {
+  MI355_SILU = 0,      /* g / (1 + exp(-g))                                         */
+  MI355_GELU = 1,      /* g * Phi(g), Phi the normal distribution function          */
+  MI355_GELU_TANH = 2  /* g / 2 * (1 + tanh(sqrt(2 / pi) * (g + 0.044715 g^3)))     */
+} mi355_activation;
+
+/* h[m][f] = act(pre[m][f]) * pre[m][F + f] from dense pre [M][2F]; pre_out (may be NULL) receives pre rounded to
+ * `dtype`.  pre_dtype: dtype, or f32 for f16 / bf16 results. */
+int mi355_gated_act(const void* pre, int pre_dtype, void* h, void* pre_out, int dtype, int64_t M, int64_t F, int act,
+                    void* stream);
+
+/* dpre[m][f] = dh * up * act'(gate), dpre[m][F + f] = dh * act(gate) with gate = pre[m][f], up = pre[m][F + f]; all
+ * dense and of `dtype`; computed in fp32 (fp64 for f64). */
+int mi355_gated_act_backward(const void* dh, const void* pre, void* dpre, int dtype, int64_t M, int64_t F, int act, void* stream);
+
+/* ---- dropout with a residual ------------------------------------------------------- */
+
+/* out[i] = residual[i] + (draw_i >= t ? x[i] * 65536 / (65536 - t) : 0), t = round(p * 65536), over n dense elements
+ * (residual NULL: 0).  draw_i is 16 bits of Philox-4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as
+ * easy as 1, 2, 3", 2011): key = the 64-bit seed, counter = offset + i / 8, bits 16 (i % 8) .. + 15 of its 128 output
+ * bits.  `rng` (device memory, two int64: seed, offset) is read by the kernel when it is not NULL, so that a captured
+ * graph draws anew after the caller has advanced it; otherwise seed and offset are used.  n elements use up
+ * (n + 7) / 8 counters.  The same draws with x = dy and no residual give the gradient.  A dropped x is not read into
+ * the result, whatever it holds. */
+int mi355_dropout_add(const void* x, const void* residual, int dtype, double p, const void* rng, int64_t seed, int64_t offset,
+                      void* out, int64_t n, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif
