@@ -23,17 +23,39 @@ constexpr int kLbMaxGroups = 256;  // row groups that leave a partial dw / db ea
 // and the weights fit the 128 registers that sixteen waves leave.  Rows of more than one wave meet in LDS, one barrier
 // per row (the slots alternate).
 constexpr int kLbTile = 1024;
+// Columns of one gradient in a partial: padded so that every partial starts on a 16-byte boundary.
+__host__ __device__ constexpr int64_t lb_ld(int64_t N) { return (N + 3) / 4 * 4; }
 constexpr int kLbTileBlocks = kNumCU;
+
+// 16 bytes at an address that is only a multiple of an element's size.
+typedef uint32_t lb_any2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t lb_any4 __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T> using LbAny = std::conditional_t<sizeof(T) == 2, lb_any2, lb_any4>;
 
 // V elements as loaded, in whole registers.
 template <typename T, int V> struct LbRaw {
-  static constexpr int R = sizeof(T) * V / 4;
+  static constexpr int R = sizeof(T) * V >= 4 ? sizeof(T) * V / 4 : 1;
   uint32_t r[R];
-  __device__ __forceinline__ void set(const VecN<T, V>& v) {
-    struct Regs { uint32_t r[R]; };
-    const Regs t = __builtin_bit_cast(Regs, v);
+  // 16-byte (fp32 weights beside two-byte rows: 32-byte) vectors at any element's address.
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (sizeof(T) * V >= 16) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) r[i] = t.r[i];
+      for (int i = 0; i < R; i += 4) {
+        const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const LbAny<T>*>(p + i * 4 / (int)sizeof(T)));
+        r[i] = v[0]; r[i + 1] = v[1]; r[i + 2] = v[2]; r[i + 3] = v[3];
+      }
+    } else if constexpr (sizeof(T) == 4) {
+      r[0] = __builtin_bit_cast(uint32_t, *p);
+    } else {
+      r[0] = __builtin_bit_cast(uint16_t, *p);
+    }
+  }
+  __device__ __forceinline__ void fill(float v) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if constexpr (sizeof(T) == 4) r[i] = __builtin_bit_cast(uint32_t, v);
+      else r[i] = (uint32_t)__builtin_bit_cast(uint16_t, static_cast<T>(v)) * 0x10001u;
+    }
   }
   __device__ __forceinline__ float get(int j) const {
     if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, r[j]);
@@ -44,9 +66,12 @@ template <typename T, int V> struct LbRaw {
 #pragma unroll
     for (int i = 0; i < R; ++i) r[i] = in ? r[i] : 0u;
   }
-  __device__ __forceinline__ void clear_unless(bool in, int j) {  // element j alone
-    if constexpr (sizeof(T) == 4) r[j] = in ? r[j] : 0u;
-    else if (!in) r[j >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+  __device__ __forceinline__ void clear_below(int first) {  // elements 0 .. first - 1
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if constexpr (sizeof(T) == 4) r[j] = j < first ? 0u : r[j];
+      else if (j < first) r[j >> 1] &= j & 1 ? 0x0000ffffu : 0xffff0000u;
+    }
   }
   __device__ __forceinline__ void keep() {
 #pragma unroll
@@ -54,62 +79,60 @@ template <typename T, int V> struct LbRaw {
   }
 };
 
-template <typename T, typename Wt, int GL, int NV, bool VEC, bool AHEAD>
+// TAIL: N is no multiple of V.  The lane whose vector would stick out of the row moves it back to end with the row; the
+// `skip` elements it then shares with its neighbour are the neighbour's.
+template <typename T, typename Wt, int V, int GL, int NV, bool TAIL>
 __global__ __launch_bounds__(kLbTile) void lb_tile_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                          const float* __restrict__ mean, const float* __restrict__ rstd,
                                                          const Wt* __restrict__ w, T* __restrict__ dx, float* __restrict__ partial,
                                                          Wt* __restrict__ dw_out, Wt* __restrict__ db_out, int64_t M, int N) {
-  constexpr int V = Vec<T>::N;
-  constexpr int G = kLbTile / GL;                     // rows a block works on at a time
-  constexpr int WPR = GL > kWave ? GL / kWave : 1;    // waves per row
+  constexpr int G = kLbTile / GL;                       // rows a block works on at a time
+  constexpr int WPR = GL > kWave ? GL / kWave : 1;      // waves per row
   constexpr int WG = GL > kWave ? G : kLbTile / kWave;  // partial sums per column that meet in LDS at the end
+  constexpr int COLS = NV * GL * V;
+  static_assert(NV * V <= 16, "32 accumulators per lane");
+  extern __shared__ __attribute__((aligned(16))) float lb_meet[];  // [dw, db][WG][COLS] when WG > 1
   __shared__ float2 red[2][kLbTile / kWave];
-  __shared__ __attribute__((aligned(16))) float meet[WG > 1 ? WG * (GL < kWave ? GL : kWave * WPR) * V : 1];
   const int t = threadIdx.x % GL, wave = threadIdx.x / kWave;
   // a row of whole waves: its number, and with it every row address, in scalar registers
   const int grp = GL >= kWave ? __builtin_amdgcn_readfirstlane(threadIdx.x / GL) : threadIdx.x / GL;
-  auto col = [&](int k, int j) { return VEC ? (k * GL + t) * V + j : (k * V + j) * GL + t; };
-  // Row data and weights as loaded.  `keep` hides them from the compiler between uses: it would otherwise carry the widened
-  // fp32 values from one use to the next (and the weights' from row to row) and spill 60 - 150 registers.
-  using Raw = LbRaw<T, V>;
-  using WRaw = LbRaw<Wt, V>;
-  WRaw gamma[NV];
-#pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    VecN<Wt, V> v;
-#pragma unroll
-    for (int j = 0; j < V; ++j) v.v[j] = w && col(k, j) < N ? w[col(k, j)] : static_cast<Wt>(1.f);
-    gamma[k].set(v);
-  }
+  // Row data and weights stay as loaded.  `keep` hides them from the compiler between uses: it would otherwise carry the
+  // widened fp32 values from one use to the next (and the weights' from row to row) and spill 60 - 150 registers.
   struct Row {
-    Raw x[NV], dy[NV];
+    LbRaw<T, V> x[NV], dy[NV];
     float mean, rstd;
   };
-  // No branches: lanes past the row and rows past the last read the nearest element that is there; one_row puts zeros in
-  // its place (with a branch per slab the compiler kept both sides of each in registers and spilled 100 of them).
+  int first[NV], skip[NV];  // first column of slab k's vector, and how many of its elements are not this lane's
+  bool in[NV];
+  LbRaw<Wt, V> gamma[NV];
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int c = (k * GL + t) * V;
+    in[k] = c < N;
+    first[k] = c + V <= N ? c : N - V;
+    skip[k] = TAIL && in[k] ? c - first[k] : 0;
+  }
+  // No branches: lanes past the row and rows past the last read what is nearest; one_row puts zeros in its place (with a
+  // branch per slab the compiler kept both sides of each in registers and spilled 100 of them).
   auto fetch = [&](int64_t row, Row& r) {
     const int64_t rc = row < M ? row : M - 1;
     r.mean = mean[rc];
     r.rstd = rstd[rc];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      VecN<T, V> xv, dv;
-      if constexpr (VEC) {  // N % V == 0: a vector is inside the row or past it
-        const int c = col(k, 0) < N ? col(k, 0) : N - V;
-        xv = ld_nt<T, V>(x + rc * N + c);
-        dv = ld_nt<T, V>(dy + rc * N + c);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int c = col(k, j) < N ? col(k, j) : N - 1;
-          xv.v[j] = x[rc * N + c];
-          dv.v[j] = dy[rc * N + c];
-        }
-      }
-      r.x[k].set(xv);
-      r.dy[k].set(dv);
+      r.x[k].load(x + rc * N + first[k]);
+      r.dy[k].load(dy + rc * N + first[k]);
     }
   };
+  const int64_t step = (int64_t)gridDim.x * G;
+  int64_t base = (int64_t)blockIdx.x * G;  // uniform over the block: every thread meets every barrier
+  Row a;
+  fetch(base + grp, a);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    if (w) gamma[k].load(w + first[k]);
+    else gamma[k].fill(1.f);
+  }
   float dw[NV][V] = {}, db[NV][V] = {};
   const float inv_n = 1.f / (float)N;
   int parity = 0;
@@ -120,26 +143,22 @@ __global__ __launch_bounds__(kLbTile) void lb_tile_kernel(const T* __restrict__ 
     float2 s = {0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      if constexpr (VEC) {
-        r.x[k].clear_unless(live && col(k, 0) < N);
-        r.dy[k].clear_unless(live && col(k, 0) < N);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          r.x[k].clear_unless(live && col(k, j) < N, j);
-          r.dy[k].clear_unless(live && col(k, j) < N, j);
-        }
-      }
+      r.x[k].clear_unless(live && in[k]);
+      r.dy[k].clear_unless(live && in[k]);
+      if constexpr (TAIL) r.x[k].keep();
+      LbRaw<T, V> d = r.dy[k];
+      if constexpr (TAIL) d.clear_below(skip[k]);
       gamma[k].keep();
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (2 * j == V) __builtin_amdgcn_sched_barrier(0);  // half a slab's temporaries at a time
-        const float d = r.dy[k].get(j), xhat = (r.x[k].get(j) - r.mean) * r.rstd;
-        const float g = d * gamma[k].get(j);
+        if (V > 4 && 2 * j == V) __builtin_amdgcn_sched_barrier(0);  // half a slab's temporaries at a time
+        float xhat = (r.x[k].get(j) - r.mean) * r.rstd;
+        if constexpr (TAIL) xhat = j < skip[k] ? 0.f : xhat;  // (0 * inf)
+        const float g = d.get(j) * gamma[k].get(j);
         s.x += g;
         s.y += g * xhat;
-        dw[k][j] += d * xhat;
-        db[k][j] += d;
+        dw[k][j] += d.get(j) * xhat;
+        db[k][j] += d.get(j);
       }
       r.x[k].keep();
       r.dy[k].keep();
@@ -165,26 +184,29 @@ __global__ __launch_bounds__(kLbTile) void lb_tile_kernel(const T* __restrict__ 
     const float m1 = s.x * inv_n, m2 = s.y * inv_n;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      VecN<T, V> o;
+      struct alignas(sizeof(T) * V) { T v[V]; } o;
       gamma[k].keep();
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        if (2 * j == V) __builtin_amdgcn_sched_barrier(0);
+        if (V > 4 && 2 * j == V) __builtin_amdgcn_sched_barrier(0);
         const float xhat = (r.x[k].get(j) - r.mean) * r.rstd;
         o.v[j] = static_cast<T>(r.rstd * (r.dy[k].get(j) * gamma[k].get(j) - m1 - xhat * m2));
-        if constexpr (!VEC)
-          if (col(k, j) < N) dx[row * N + col(k, j)] = o.v[j];
       }
-      if constexpr (VEC)
-        if (col(k, 0) < N) st_nt<T, V>(dx + row * N + col(k, 0), o);
+      T* out = dx + row * N + first[k];
+      if constexpr (V == 1) {
+        if (in[k]) *out = o.v[0];
+      } else if (in[k] && (!TAIL || skip[k] == 0)) {
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4, o), reinterpret_cast<LbAny<T>*>(out));
+      } else if (TAIL && in[k]) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j >= skip[k]) out[j] = o.v[j];
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  const int64_t step = (int64_t)gridDim.x * G;
-  int64_t base = (int64_t)blockIdx.x * G;  // uniform over the block: every thread meets every barrier
-  if constexpr (AHEAD) {
-    Row a, b;
-    fetch(base + grp, a);
+  if constexpr (NV <= 2) {
+    Row b;
     while (base < M) {  // two rows per trip, the two register sets trading places
       fetch(base + step + grp, b);
       one_row(base + grp, a);
@@ -194,50 +216,77 @@ __global__ __launch_bounds__(kLbTile) void lb_tile_kernel(const T* __restrict__ 
       one_row(base + grp, b);
       base += step;
     }
-  } else {
-    for (; base < M; base += step) {
-      Row a;
-      fetch(base + grp, a);
+  } else {  // no room for a second row
+    while (base < M) {
       one_row(base + grp, a);
+      base += step;
+      fetch(base + grp, a);
     }
   }
   if (partial == nullptr && dw_out == nullptr && db_out == nullptr) return;
-  // This block's dw, then its db, V x GL columns at a time: the row groups' values meet in LDS (groups smaller than a wave
-  // first by exchanges inside it) and leave as one partial, or as the result when this is the only block.
-  constexpr int COLS = GL * V;
-  auto leave = [&](float (&acc)[NV][V], float* part, Wt* out) {
+  // This block's dw and db: the row groups' values meet in LDS (groups smaller than a wave first by exchanges inside it) and
+  // leave as one partial [dw | db], each padded to lb_ld(N) columns, or as the result when this is the only block.
+  const int64_t ld_n = lb_ld(N);
+  float* part = partial + (int64_t)blockIdx.x * 2 * ld_n;
+  if constexpr (WG == 1) {
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-      auto put = [&](int c, float v) {
-        if (c >= N) return;
-        if (partial != nullptr) part[c] = v;
-        else if (out != nullptr) out[c] = static_cast<Wt>(v);
-      };
-      if constexpr (WG == 1) {
+    for (int k = 0; k < NV; ++k)
 #pragma unroll
-        for (int j = 0; j < V; ++j) put(col(k, j), acc[k][j]);
-      } else {
-        __syncthreads();  // the buffer's last values have been read
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float v = acc[k][j];
-#pragma unroll
-          for (int d = GL; d < kWave; d *= 2) v += __shfl_xor(v, d, kWave);
-          if (GL >= kWave || threadIdx.x % kWave < GL) meet[(GL >= kWave ? grp : wave) * COLS + (VEC ? t * V + j : j * GL + t)] = v;
-        }
-        __syncthreads();
-        for (int c = threadIdx.x; c < COLS; c += kLbTile) {
-          float v = 0.f;
-#pragma unroll
-          for (int g = 0; g < WG; ++g) v += meet[g * COLS + c];
-          put(k * COLS + c, v);
+      for (int j = 0; j < V; ++j) {
+        const int c = first[k] + j;
+        if (!in[k] || (TAIL && j < skip[k])) continue;
+        if (partial != nullptr) {
+          part[c] = dw[k][j];
+          part[ld_n + c] = db[k][j];
+        } else {
+          if (dw_out != nullptr) dw_out[c] = static_cast<Wt>(dw[k][j]);
+          if (db_out != nullptr) db_out[c] = static_cast<Wt>(db[k][j]);
         }
       }
+  } else {
+    auto park = [&](float (&acc)[NV][V], int which) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+          for (int d = GL; d < kWave; d *= 2) acc[k][j] += __shfl_xor(acc[k][j], d, kWave);
+        if (!in[k] || (GL < kWave && threadIdx.x % kWave >= GL)) continue;
+        float* dst = lb_meet + (which * WG + (GL >= kWave ? grp : wave)) * COLS + first[k];
+        if constexpr (TAIL || V == 1) {
+#pragma unroll
+          for (int j = 0; j < V; ++j)
+            if (j >= skip[k]) dst[j] = acc[k][j];
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(dst + j) = float4{acc[k][j], acc[k][j + 1], acc[k][j + 2], acc[k][j + 3]};
+        }
+      }
+    };
+    park(dw, 0);
+    park(db, 1);
+    __syncthreads();
+    const int quads = (int)ld_n / 4;
+    for (int q = threadIdx.x; q < 2 * quads; q += kLbTile) {
+      const int which = q >= quads, c = 4 * (which ? q - quads : q);
+      float4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int g = 0; g < WG; ++g) {
+        const float4 o = *reinterpret_cast<const float4*>(lb_meet + (which * WG + g) * COLS + c);
+        v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+      }
+      if (partial != nullptr) {  // (columns past N are padding: never read back)
+        *reinterpret_cast<float4*>(part + which * ld_n + c) = v;
+      } else {
+        Wt* out = which ? db_out : dw_out;
+        const float e[4] = {v.x, v.y, v.z, v.w};
+        if (out != nullptr)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c + j < N) out[c + j] = static_cast<Wt>(e[j]);
+      }
     }
-  };
-  float* part = partial + (int64_t)blockIdx.x * 2 * N;
-  leave(dw, part, dw_out);
-  leave(db, part + N, db_out);
+  }
 }
 
 // sums[row] = {mean_N(g), mean_N(g xhat)}.
@@ -265,7 +314,7 @@ __global__ __launch_bounds__(kLbBlock) void lb_row_means_kernel(const T* __restr
   }
 }
 
-// One column per thread, blockIdx.y = row group; partial[group][0 / 1][N] = the group's dw / db.
+// One column per thread, blockIdx.y = row group; partial[group][0 / 1][lb_ld(N)] = the group's dw / db.
 template <typename T, typename Wt, typename S>
 __global__ __launch_bounds__(kLbBlock) void lb_columns_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                              const S* __restrict__ mean, const S* __restrict__ rstd,
@@ -285,8 +334,8 @@ __global__ __launch_bounds__(kLbBlock) void lb_columns_kernel(const T* __restric
     if (dx) dx[r * N + c] = static_cast<T>(rs * (d * gamma - sums[2 * r] - xhat * sums[2 * r + 1]));
   }
   if (partial) {
-    partial[(int64_t)blockIdx.y * 2 * N + c] = dw;
-    partial[(int64_t)blockIdx.y * 2 * N + N + c] = db;
+    partial[(int64_t)blockIdx.y * 2 * lb_ld(N) + c] = dw;
+    partial[((int64_t)blockIdx.y * 2 + 1) * lb_ld(N) + c] = db;
   }
 }
 
@@ -296,34 +345,27 @@ __global__ __launch_bounds__(kLbBlock) void lb_finish_kernel(const S* __restrict
                                                             int64_t N, int groups) {
   __shared__ S part[16][64];
   const int q = threadIdx.x / 16, l = threadIdx.x % 16;
-  const int64_t c0 = (int64_t)blockIdx.x * 64 + 4 * l;  // of the 2N columns [dw | db]
+  const int64_t ld_n = lb_ld(N), c0 = (int64_t)blockIdx.x * 64 + 4 * l;  // of the 2 ld_n columns [dw | db]
   S s[4] = {};
-  if (N % 2 == 0) {  // every group of four columns starts on a 16-byte boundary (of fp32) and is inside or outside as a whole
-    if (c0 < 2 * N) {
+  if (c0 < 2 * ld_n) {
 #pragma unroll 8
-      for (int g = q; g < groups; g += 16) {
-        const VecN<S, 4> v = ld<S, 4>(partial + (int64_t)g * 2 * N + c0);
+    for (int g = q; g < groups; g += 16) {
+      const VecN<S, 4> v = ld<S, 4>(partial + (int64_t)g * 2 * ld_n + c0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] += v.v[j];
-      }
+      for (int j = 0; j < 4; ++j) s[j] += v.v[j];
     }
-  } else {
-#pragma unroll 4
-    for (int g = q; g < groups; g += 16)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (c0 + j < 2 * N) s[j] += partial[(int64_t)g * 2 * N + c0 + j];
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) part[q][4 * l + j] = s[j];
   __syncthreads();
   const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (threadIdx.x >= 64 || c >= 2 * N) return;
+  const int64_t col = c < ld_n ? c : c - ld_n;
+  if (threadIdx.x >= 64 || c >= 2 * ld_n || col >= N) return;
   S sum = 0;
 #pragma unroll
   for (int i = 0; i < 16; ++i) sum += part[i][threadIdx.x];
-  Wt* out = c < N ? dw : db;
-  if (out) out[c < N ? c : c - N] = static_cast<Wt>(sum);
+  Wt* out = c < ld_n ? dw : db;
+  if (out) out[col] = static_cast<Wt>(sum);
 }
 
 struct LbPlan {
@@ -342,8 +384,8 @@ static LbPlan lb_plan(int64_t M, int64_t N) {
   return LbPlan{(M + per - 1) / per, per};
 }
 
-// Lanes per row and slabs per lane of the tile kernel; lanes == 0: the general path.  Two-byte rows take at most two slabs
-// of 8 elements per lane, fp32 rows two of 4, or four without the row ahead beyond 8 K elements.
+// Lanes per row and slabs per lane of the tile kernel; lanes == 0: the general path.  A slab is one 16-byte vector per lane
+// (single elements for rows shorter than that); two-byte rows take at most two, fp32 rows four.
 struct LbTile {
   int lanes, slabs;
 };
@@ -363,31 +405,43 @@ static int64_t lb_tile_blocks(int64_t M, const LbTile& p) {
   return need < kLbTileBlocks ? need : kLbTileBlocks;
 }
 
+template <typename T, typename Wt, int V, int GL, int NV, bool TAIL>
+static int launch_lb_tile(int64_t blocks, const T* dy, const T* x, const float* mean, const float* rstd, const Wt* w, T* dx, float* partial,
+                          Wt* dw, Wt* db, int64_t M, int64_t N, hipStream_t st) {
+  constexpr int WG = GL > kWave ? kLbTile / GL : kLbTile / kWave;
+  constexpr int bytes = WG > 1 ? 2 * WG * NV * GL * V * (int)sizeof(float) : 0;
+  const auto kern = lb_tile_kernel<T, Wt, V, GL, NV, TAIL>;
+  if (bytes > 48 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) return set_error(MI355_ERR_LAUNCH, "mi355_layer_norm_backward: cannot reserve %d bytes of LDS: %s", bytes, hipGetErrorString(e));
+  }
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(kLbTile), bytes, st, dy, x, mean, rstd, w, dx, partial, dw, db, M, (int)N);
+  return check_launch("mi355_layer_norm_backward");
+}
+
 template <typename T, typename Wt>
-static bool run_lb_tile(const T* dy, const T* x, const float* mean, const float* rstd, const Wt* w, T* dx, Wt* dw, Wt* db, int64_t M,
-                        int64_t N, float* ws, hipStream_t st) {
-  const LbTile p = lb_tile<T>(N);
-  if (p.lanes == 0) return false;
+static int run_lb_tile(const LbTile& p, const T* dy, const T* x, const float* mean, const float* rstd, const Wt* w, T* dx, Wt* dw, Wt* db,
+                       int64_t M, int64_t N, float* ws, hipStream_t st) {
+  constexpr int V = 16 / sizeof(T);
   const int64_t blocks = lb_tile_blocks(M, p);
-  const bool params = dw != nullptr || db != nullptr;
-  float* partial = params && blocks > 1 ? ws : nullptr;
-  const bool vec = N % Vec<T>::N == 0 && aligned16(dy) && aligned16(x) && aligned16(dx);
-  auto go = [&](auto gl, auto nv) {
-    constexpr int GL = decltype(gl)::value, NV = decltype(nv)::value;
-    if (vec) hipLaunchKernelGGL((lb_tile_kernel<T, Wt, GL, NV, true, (NV <= 2)>), dim3((unsigned)blocks), dim3(kLbTile), 0, st, dy, x, mean, rstd, w, dx, partial, dw, db, M, (int)N);
-    else hipLaunchKernelGGL((lb_tile_kernel<T, Wt, GL, NV, false, false>), dim3((unsigned)blocks), dim3(kLbTile), 0, st, dy, x, mean, rstd, w, dx, partial, dw, db, M, (int)N);
-  };
-  using std::integral_constant;
-#define MI355_LB_TILE(GL_, NV_) \
-  if (p.lanes == GL_ && p.slabs == NV_) go(integral_constant<int, GL_>(), integral_constant<int, NV_>());
-  MI355_LB_TILE(8, 1) MI355_LB_TILE(16, 1) MI355_LB_TILE(32, 1)
-  MI355_LB_TILE(64, 1) MI355_LB_TILE(128, 1) MI355_LB_TILE(256, 1) MI355_LB_TILE(512, 1) MI355_LB_TILE(1024, 1)
-  MI355_LB_TILE(64, 2) MI355_LB_TILE(128, 2) MI355_LB_TILE(256, 2) MI355_LB_TILE(512, 2) MI355_LB_TILE(1024, 2)
-  if constexpr (sizeof(T) == 4) MI355_LB_TILE(1024, 4)
+  float* partial = (dw != nullptr || db != nullptr) && blocks > 1 ? ws : nullptr;
+  int rc = MI355_OK;
+#define MI355_LB_TILE(GL_, NV_)                                                                                              \
+  if (p.lanes == GL_ && p.slabs == NV_)                                                                                       \
+    rc = N % V == 0 ? launch_lb_tile<T, Wt, V, GL_, NV_, false>(blocks, dy, x, mean, rstd, w, dx, partial, dw, db, M, N, st)  \
+                    : launch_lb_tile<T, Wt, V, GL_, NV_, true>(blocks, dy, x, mean, rstd, w, dx, partial, dw, db, M, N, st);
+  if (N < V) {
+    rc = launch_lb_tile<T, Wt, 1, 8, 1, false>(blocks, dy, x, mean, rstd, w, dx, partial, dw, db, M, N, st);
+  } else {
+    MI355_LB_TILE(8, 1) MI355_LB_TILE(16, 1) MI355_LB_TILE(32, 1)
+    MI355_LB_TILE(64, 1) MI355_LB_TILE(128, 1) MI355_LB_TILE(256, 1) MI355_LB_TILE(512, 1) MI355_LB_TILE(1024, 1)
+    MI355_LB_TILE(64, 2) MI355_LB_TILE(128, 2) MI355_LB_TILE(256, 2) MI355_LB_TILE(512, 2) MI355_LB_TILE(1024, 2)
+    if constexpr (sizeof(T) == 4) MI355_LB_TILE(1024, 4)
+  }
 #undef MI355_LB_TILE
-  if (partial)
-    hipLaunchKernelGGL((lb_finish_kernel<Wt, float>), dim3((unsigned)((2 * N + 63) / 64)), dim3(kLbBlock), 0, st, partial, dw, db, N, (int)blocks);
-  return true;
+  if (rc != MI355_OK || partial == nullptr) return rc;
+  hipLaunchKernelGGL((lb_finish_kernel<Wt, float>), dim3((unsigned)((2 * lb_ld(N) + 63) / 64)), dim3(kLbBlock), 0, st, partial, dw, db, N, (int)blocks);
+  return check_launch("mi355_layer_norm_backward");
 }
 
 template <typename T, typename Wt, typename S>
@@ -397,18 +451,20 @@ static int run_lb(const void* dyv, const void* xv, const void* mv, const void* r
   const S *mean = static_cast<const S*>(mv), *rstd = static_cast<const S*>(rv);
   const Wt* w = static_cast<const Wt*>(wv);
   if constexpr (!std::is_same<T, double>::value) {
-    if (run_lb_tile<T, Wt>(dy, x, mean, rstd, w, static_cast<T*>(dxv), static_cast<Wt*>(dwv), static_cast<Wt*>(dbv), M, N, static_cast<float*>(ws), st))
-      return check_launch("mi355_layer_norm_backward");
+    const LbTile tile = lb_tile<T>(N);
+    if (tile.lanes != 0)
+      return run_lb_tile<T, Wt>(tile, dy, x, mean, rstd, w, static_cast<T*>(dxv), static_cast<Wt*>(dwv), static_cast<Wt*>(dbv), M, N,
+                                static_cast<float*>(ws), st);
   }
-  S* sums = static_cast<S*>(ws);
-  S* partial = (dwv != nullptr || dbv != nullptr) ? sums + 2 * M : nullptr;
+  S* partial = (dwv != nullptr || dbv != nullptr) ? static_cast<S*>(ws) : nullptr;
+  S* sums = static_cast<S*>(ws) + lb_plan(M, N).groups * 2 * lb_ld(N);  // behind the partials
   const LbPlan p = lb_plan(M, N);
   if (dxv != nullptr)
     hipLaunchKernelGGL((lb_row_means_kernel<T, Wt, S>), dim3((unsigned)grid_for(M, 1, kNumCU * 32)), dim3(kLbBlock), 0, st, dy, x, mean, rstd, w, sums, M, N);
   hipLaunchKernelGGL((lb_columns_kernel<T, Wt, S>), dim3((unsigned)((N + kLbBlock - 1) / kLbBlock), (unsigned)p.groups), dim3(kLbBlock), 0, st, dy,
                      x, mean, rstd, w, sums, static_cast<T*>(dxv), partial, M, N, p.rows_per_group);
   if (partial)
-    hipLaunchKernelGGL((lb_finish_kernel<Wt, S>), dim3((unsigned)((2 * N + 63) / 64)), dim3(kLbBlock), 0, st, partial,
+    hipLaunchKernelGGL((lb_finish_kernel<Wt, S>), dim3((unsigned)((2 * lb_ld(N) + 63) / 64)), dim3(kLbBlock), 0, st, partial,
                        static_cast<Wt*>(dwv), static_cast<Wt*>(dbv), N, (int)p.groups);
   return check_launch("mi355_layer_norm_backward");
 }
@@ -420,8 +476,8 @@ using namespace mi355;
 extern "C" int64_t mi355_layer_norm_backward_workspace_bytes(int64_t M, int64_t N, int dtype) {
   if (M <= 0 || N <= 0 || dtype_size(dtype) == 0) return 0;
   const LbTile p = dtype == MI355_F32 ? lb_tile<float>(N) : dtype == MI355_F64 ? lb_tile<double>(N) : lb_tile<bf16_t>(N);
-  if (p.lanes != 0) return lb_tile_blocks(M, p) * 2 * N * 4;
-  return (2 * M + lb_plan(M, N).groups * 2 * N) * (dtype == MI355_F64 ? 8 : 4);
+  if (p.lanes != 0) return lb_tile_blocks(M, p) * 2 * lb_ld(N) * 4;
+  return (2 * M + lb_plan(M, N).groups * 2 * lb_ld(N)) * (dtype == MI355_F64 ? 8 : 4);
 }
 
 extern "C" int mi355_layer_norm_backward(const void* dy, const void* x, int dtype, const void* mean, const void* rstd,
