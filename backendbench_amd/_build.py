@@ -25,6 +25,7 @@ SOURCES = [
     "layernorm.hip",
     "layernorm_bwd.hip",
     "gated.hip",
+    "gated_x16.hip",
     "dropout.hip",
     "index.hip",
     "gemm.hip",
@@ -99,7 +100,7 @@ def ablate_lib_path(bits: int) -> Path:
 
 def build_ablate(bits: int, verbose: bool = True) -> Path:
     """A measurement build of the GEMM sources with -DMI355_X16_ABLATE=<bits>: parts of the 16x16x32
-    kernel's K loop or epilogue left out (bit list beside the macro in csrc/gemm_x16.hip).  Its results
+    kernel's K loop or epilogue left out (bit list beside the macro in csrc/gemm_x16.h).  Its results
     are wrong; `bench.py --only-op C3.mm_down --ablate <bits>` times it to show what each part costs."""
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
     objs = []

@@ -9,25 +9,67 @@ __device__ __forceinline__ float gate_exp(float v) { return expf(v); }
 __device__ __forceinline__ double gate_exp(double v) { return exp(v); }
 __device__ __forceinline__ float gate_erfc(float v) { return erfcf(v); }
 __device__ __forceinline__ double gate_erfc(double v) { return erfc(v); }
+__device__ __forceinline__ float gate_div(float a, float b) { return a / b; }
+__device__ __forceinline__ double gate_div(double a, double b) { return a / b; }
+
+// float arithmetic whose result is rounded to 16 bits: the hardware's exp2 and reciprocal (1 ulp each; the exponential's
+// argument is rounded once more, |v| 2^-24 of relative error) instead of the library's exact-rounding sequences.
+struct GateHalf {
+  float v;
+  __device__ __forceinline__ GateHalf(float f) : v(f) {}
+  __device__ __forceinline__ operator float() const { return v; }
+};
+__device__ __forceinline__ float gate_exp(GateHalf a) { return __builtin_amdgcn_exp2f(a.v * 1.44269504088896340736f); }
+// erfc(v) = t P(t) exp(-v^2), t = 1 / (1 + 0.46 v), for v >= 0: P of degree 7 fitted here to erfc(v) exp(v^2) / t over all of
+// t in (0, 1] for the smallest relative error, 6.8e-7, so the far tail keeps its digits; erfc(-v) = 2 - erfc(v).
+__device__ __forceinline__ float gate_erfc(GateHalf a) {
+  const float v = __builtin_fabsf(a.v), t = __builtin_amdgcn_rcpf(1.f + 0.46f * v);
+  float p = 0.0677143769f;
+  p = __builtin_fmaf(p, t, -0.226629397f);
+  p = __builtin_fmaf(p, t, 0.169191163f);
+  p = __builtin_fmaf(p, t, 0.0526105011f);
+  p = __builtin_fmaf(p, t, 0.186847832f);
+  p = __builtin_fmaf(p, t, 0.231181876f);
+  p = __builtin_fmaf(p, t, 0.259557266f);
+  p = __builtin_fmaf(p, t, 0.259527059f);
+  const float e = p * t * __builtin_amdgcn_exp2f(v * v * -1.44269504088896340736f);
+  return a.v < 0.f ? 2.f - e : e;
+}
+__device__ __forceinline__ float gate_div(GateHalf a, float b) { return a.v * __builtin_amdgcn_rcpf(b); }
 
 // 1 / (1 + exp(-v)) from exp(-|v|): no overflow, and full relative accuracy on the negative side.
-template <typename A> __device__ __forceinline__ A gate_sigmoid(A v) {
-  const A e = gate_exp(v < A(0) ? v : -v);
-  return (v < A(0) ? e : A(1)) / (A(1) + e);
+template <typename A, typename F> __device__ __forceinline__ F gate_sigmoid(F v) {
+  const F e = gate_exp(A(v < F(0) ? v : -v));
+  return gate_div(A(v < F(0) ? e : F(1)), F(1) + e);
 }
 // act(g) = g * q(g) for all three: q = sigmoid(g), Phi(g), or (1 + tanh z) / 2 = sigmoid(2 z).
 // Phi comes from erfc, which keeps its relative accuracy in the negative tail.
-template <int ACT, typename A> __device__ __forceinline__ A gate_q(A g) {
-  if constexpr (ACT == MI355_SILU) return gate_sigmoid(g);
-  if constexpr (ACT == MI355_GELU) return A(0.5) * gate_erfc(g * A(-0.70710678118654752440));
-  return gate_sigmoid(A(1.59576912160573071176) * (g + A(0.044715) * g * g * g));  // 2 sqrt(2 / pi) (g + 0.044715 g^3)
+template <int ACT, typename A, typename F> __device__ __forceinline__ F gate_q(F g) {
+  if constexpr (ACT == MI355_SILU) return gate_sigmoid<A>(g);
+  if constexpr (ACT == MI355_GELU) return F(0.5) * gate_erfc(A(g * F(-0.70710678118654752440)));
+  return gate_sigmoid<A>(F(1.59576912160573071176) * (g + F(0.044715) * g * g * g));  // 2 sqrt(2 / pi) (g + 0.044715 g^3)
 }
 // act'(g) given q = gate_q(g).
-template <int ACT, typename A> __device__ __forceinline__ A gate_grad(A g, A q) {
-  if constexpr (ACT == MI355_SILU) return q * (A(1) + g * (A(1) - q));
-  if constexpr (ACT == MI355_GELU) return q + g * gate_exp(A(-0.5) * g * g) * A(0.39894228040143267794);
-  const A d = q * (A(1) - q);  // 0 far out, where g * g may already be infinite
-  return d == A(0) ? q : q + g * d * A(1.59576912160573071176) * (A(1) + A(3 * 0.044715) * g * g);
+template <int ACT, typename A, typename F> __device__ __forceinline__ F gate_grad(F g, F q) {
+  if constexpr (ACT == MI355_SILU) return q * (F(1) + g * (F(1) - q));
+  if constexpr (ACT == MI355_GELU) return q + g * gate_exp(A(F(-0.5) * g * g)) * F(0.39894228040143267794);
+  const F d = q * (F(1) - q);  // 0 far out, where g * g may already be infinite
+  return d == F(0) ? q : q + g * d * F(1.59576912160573071176) * (F(1) + F(3 * 0.044715) * g * g);
 }
+// The arithmetic for results of type T.
+template <typename T> using GateMath = std::conditional_t<sizeof(T) == 2, GateHalf, typename OpMath<T>::type>;
+
+// One gated projection: x [M][K], weight [2F][K] (gate rows, then up rows), both K-contiguous; h [M][F]; pre [M][2F] or null.
+struct GatedArgs {
+  const void* x;
+  const void* w;
+  void* h;
+  void* pre;
+  int64_t x_rs, w_rs, M, F, K;
+  int act, dtype;
+};
+// gated_x16.hip
+bool gated_x16_takes(const GatedArgs& a);
+int launch_gated_x16(const GatedArgs& a, hipStream_t st);
 
 }  // namespace mi355

@@ -18,7 +18,7 @@ __global__ __launch_bounds__(256) void gated_act_kernel(const P* __restrict__ pr
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const A ga = static_cast<A>(g.v[j]), ua = static_cast<A>(u.v[j]);
-      r.v[j] = static_cast<T>(ga * gate_q<ACT, A>(ga) * ua);
+      r.v[j] = static_cast<T>(ga * gate_q<ACT, GateMath<T>>(ga) * ua);
       if constexpr (SAVE) {
         sg.v[j] = static_cast<T>(ga);
         su.v[j] = static_cast<T>(ua);
@@ -44,8 +44,8 @@ __global__ __launch_bounds__(256) void gated_act_backward_kernel(const T* __rest
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const A ga = static_cast<A>(g.v[j]), ua = static_cast<A>(u.v[j]), da = static_cast<A>(d.v[j]);
-      const A q = gate_q<ACT, A>(ga);
-      dg.v[j] = static_cast<T>(da * ua * gate_grad<ACT, A>(ga, q));
+      const A q = gate_q<ACT, GateMath<T>>(ga);
+      dg.v[j] = static_cast<T>(da * ua * gate_grad<ACT, GateMath<T>>(ga, q));
       du.v[j] = static_cast<T>(da * (ga * q));
     }
     st<T, V>(dpre + m * 2 * F + f, dg);
@@ -125,4 +125,21 @@ extern "C" int mi355_gated_act_backward(const void* dh, const void* pre, void* d
   MI355_REQUIRE(dh != nullptr && pre != nullptr && dpre != nullptr, "mi355_gated_act_backward: NULL data pointer");
   MI355_DISPATCH_FLOAT(dtype, "mi355_gated_act_backward",
                        return run_gated_act_backward<T>(dh, pre, dpre, M, F, act, static_cast<hipStream_t>(stream)));
+}
+
+extern "C" int mi355_gated_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, void* h, void* pre, int64_t M, int64_t F,
+                                  int64_t K, int act, int dtype, void* stream) {
+  MI355_REQUIRE(M >= 0 && F >= 0 && K >= 0, "mi355_gated_linear: negative extent");
+  MI355_REQUIRE(act >= MI355_SILU && act <= MI355_GELU_TANH, "mi355_gated_linear: unknown activation %d", act);
+  if (M == 0 || F == 0) return MI355_OK;
+  MI355_REQUIRE(x != nullptr && weight != nullptr && h != nullptr, "mi355_gated_linear: NULL data pointer");
+  MI355_REQUIRE((x_rs >= K || M == 1) && w_rs >= K, "mi355_gated_linear: rows overlap (strides %lld, %lld for K = %lld)", (long long)x_rs,
+                (long long)w_rs, (long long)K);
+  const GatedArgs a{x, weight, h, pre, M == 1 ? K : x_rs, w_rs, M, F, K, act, dtype};
+  const bool half = dtype == MI355_BF16 || dtype == MI355_F16;
+  const bool rows16 = a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && aligned16(x) && aligned16(weight);
+  const bool fits = M < (1 << 30) && F < (1 << 29) && K < (1 << 30);
+  if (half && rows16 && fits && gated_x16_takes(a)) return launch_gated_x16(a, static_cast<hipStream_t>(stream));
+  return set_error(MI355_ERR_UNSUPPORTED, "mi355_gated_linear: no single kernel for M=%lld F=%lld K=%lld %s", (long long)M, (long long)F,
+                   (long long)K, dtype_name(dtype));
 }

@@ -96,8 +96,8 @@ _ready = set()  # devices mi355_init() has accepted
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def launch(name, *args):
-    """Call one C entry point with the current stream appended; raise on failure."""
+def _enqueue(name, args):
+    """Call one C entry point with the current stream appended; its status."""
     for w in _flag_words:
         if w.value:
             poll_index_errors()
@@ -109,9 +109,27 @@ def launch(name, *args):
     if dev not in _ready:
         _lib.init_device(dev)  # refuses a GPU the launch heuristics are not built for
         _ready.add(dev)
-    rc = fn(*args, _lib.current_stream_handle())
+    return fn(*args, _lib.current_stream_handle())
+
+
+def launch(name, *args):
+    """Call one C entry point with the current stream appended; raise on failure."""
+    rc = _enqueue(name, args)
     if rc != 0:
         _lib.check(rc)
+
+
+_UNSUPPORTED = -2  # MI355_ERR_UNSUPPORTED
+
+
+def try_launch(name, *args):
+    """launch(), but False instead of an error when the entry point has no kernel for the operands (nothing was launched)."""
+    rc = _enqueue(name, args)
+    if rc == _UNSUPPORTED:
+        return False
+    if rc != 0:
+        _lib.check(rc)
+    return True
 
 
 def row_major_strides(shape):

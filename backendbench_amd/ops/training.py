@@ -8,7 +8,8 @@ a call of the operator that computes it.  Arguments are checked before anything 
 import torch
 
 from .. import _lib
-from ._common import (cast, copy_into, dense, device_managed, launch, new_dense, new_result, on_device_of_arguments, prod)
+from ._common import (cast, copy_into, dense, device_managed, launch, new_dense, new_result, on_device_of_arguments, prod,
+                      try_launch)
 from .elementwise import _store_result as store_result
 from .elementwise import tuple_out_variant
 from .matmul import _gemm, _gemm_f32out
@@ -132,6 +133,25 @@ def gated_linear(input, weight, activation="silu", save_pre=False):
     return _gated_linear(input, weight, activation, bool(save_pre))
 
 
+_PAD_ROWS = 64  # more rows than this are worth a zero-padded copy of a weight whose rows the kernels cannot take
+
+
+def _gated_fused(x, weight, h, pre, act):
+    """The one-kernel form on x [M, K]; False when there is none for these operands (nothing was launched)."""
+    M, K = x.shape
+    if weight.stride(1) != 1 and K > 1:
+        weight = dense(weight)
+    if M > _PAD_ROWS and (K % 128 or K < 256 or weight.stride(0) % 8 or weight.data_ptr() % 16 or x.data_ptr() % 16):
+        # copied once into rows of a multiple of 128 (exact: the pad adds 0 * 0 terms)
+        Kp = max((K + 127) // 128 * 128, 256)
+        both = torch.zeros((M + weight.shape[0], Kp), dtype=x.dtype, device=x.device)
+        copy_into(both[:M, :K], x)
+        copy_into(both[M:, :K], weight)
+        x, weight = both[:M], both[M:]
+    return try_launch("mi355_gated_linear", x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), h.data_ptr(),
+                      pre.data_ptr() if pre is not None else None, M, weight.shape[0] // 2, x.shape[1], act, _lib.dtype_code(x.dtype))
+
+
 @device_managed
 @on_device_of_arguments
 def _gated_linear(input, weight, activation, save_pre):
@@ -143,17 +163,18 @@ def _gated_linear(input, weight, activation, save_pre):
         return (h, torch.zeros(lead + [2 * F], dtype=dtype, device=device)) if save_pre else h
     h = new_dense(lead + [F], dtype, device)
     pre = new_dense(lead + [2 * F], dtype, device) if save_pre else None
+    act = _ACTIVATIONS[activation]
     x = dense(input).view(M, K)
     if dtype in _HALF:
-        wide = _gemm_f32out(x, weight.t(), None, 1.0, 0.0)
-        saved = pre
+        if _gated_fused(x, weight, h, pre, act):
+            return (h, pre) if save_pre else h
+        wide, saved = _gemm_f32out(x, weight.t(), None, 1.0, 0.0), pre
     else:
-        wide = _gemm(x, weight.t(), None, 1.0, 0.0)
-        saved = None
+        wide, saved = _gemm(x, weight.t(), None, 1.0, 0.0), None
         if save_pre:
             pre = wide.view(lead + [2 * F])
     launch("mi355_gated_act", wide.data_ptr(), _lib.dtype_code(wide.dtype), h.data_ptr(),
-           saved.data_ptr() if saved is not None else None, _lib.dtype_code(dtype), M, F, _ACTIVATIONS[activation])
+           saved.data_ptr() if saved is not None else None, _lib.dtype_code(dtype), M, F, act)
     return (h, pre) if save_pre else h
 
 

@@ -36,6 +36,13 @@ typedef enum mi355_activation {
   MI355_GELU_TANH = 2  /* g / 2 * (1 + tanh(sqrt(2 / pi) * (g + 0.044715 g^3)))     */
 } mi355_activation;
 
+/* h = act(x Wg^T) * (x Wu^T) in one kernel: x [M][K] with rows x_rs apart, weight [2F][K] = [Wg; Wu] with rows w_rs
+ * apart, both unit-stride along K; h [M][F] dense; pre (may be NULL) receives the pre-activations [M][2F], dense.  All of
+ * `dtype`.  Products accumulate in fp32; the activation takes the unrounded sums.  For f16 / bf16 with 16-byte aligned
+ * rows of K % 128 == 0, K >= 256; otherwise MI355_ERR_UNSUPPORTED with nothing launched (a product and mi355_gated_act do it). */
+int mi355_gated_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, void* h, void* pre, int64_t M, int64_t F,
+                       int64_t K, int act, int dtype, void* stream);
+
 /* h[m][f] = act(pre[m][f]) * pre[m][F + f] from dense pre [M][2F]; pre_out (may be NULL) receives pre rounded to
  * `dtype`.  pre_dtype: dtype, or f32 for f16 / bf16 results. */
 int mi355_gated_act(const void* pre, int pre_dtype, void* h, void* pre_out, int dtype, int64_t M, int64_t F, int act,
