@@ -26,6 +26,7 @@ SOURCES = [
     "layernorm_bwd.hip",
     "gated.hip",
     "gated_x16.hip",
+    "gated_rows.hip",
     "dropout.hip",
     "index.hip",
     "gemm.hip",

@@ -139,6 +139,7 @@ extern "C" int mi355_gated_linear(const void* x, int64_t x_rs, const void* weigh
   const bool half = dtype == MI355_BF16 || dtype == MI355_F16;
   const bool rows16 = a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && aligned16(x) && aligned16(weight);
   const bool fits = M < (1 << 30) && F < (1 << 29) && K < (1 << 30);
+  if (half && fits && M <= kGatedRows) return launch_gated_rows(a, static_cast<hipStream_t>(stream));
   if (half && rows16 && fits && gated_x16_takes(a)) return launch_gated_x16(a, static_cast<hipStream_t>(stream));
   return set_error(MI355_ERR_UNSUPPORTED, "mi355_gated_linear: no single kernel for M=%lld F=%lld K=%lld %s", (long long)M, (long long)F,
                    (long long)K, dtype_name(dtype));

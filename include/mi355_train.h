@@ -38,8 +38,9 @@ typedef enum mi355_activation {
 
 /* h = act(x Wg^T) * (x Wu^T) in one kernel: x [M][K] with rows x_rs apart, weight [2F][K] = [Wg; Wu] with rows w_rs
  * apart, both unit-stride along K; h [M][F] dense; pre (may be NULL) receives the pre-activations [M][2F], dense.  All of
- * `dtype`.  Products accumulate in fp32; the activation takes the unrounded sums.  For f16 / bf16 with 16-byte aligned
- * rows of K % 128 == 0, K >= 256; otherwise MI355_ERR_UNSUPPORTED with nothing launched (a product and mi355_gated_act do it). */
+ * `dtype`.  Products accumulate in fp32; the activation takes the unrounded sums.  For f16 / bf16: up to 64 rows
+ * with any K, strides and alignment; more rows with 16-byte aligned rows of K % 128 == 0, K >= 256.  Otherwise
+ * MI355_ERR_UNSUPPORTED with nothing launched (a product and mi355_gated_act do it). */
 int mi355_gated_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, void* h, void* pre, int64_t M, int64_t F,
                        int64_t K, int act, int dtype, void* stream);
 
