@@ -71,6 +71,8 @@ struct GatedArgs {
 // gated_x16.hip
 bool gated_x16_takes(const GatedArgs& a);
 int launch_gated_x16(const GatedArgs& a, hipStream_t st);
+// gemm.hip: 128 rows by 64 features per workgroup; K % 64 == 0, 16-byte aligned rows
+int launch_gated_small2(const GatedArgs& a, hipStream_t st);
 // gated_rows.hip: at most kGatedRows rows, any K, strides and alignment
 constexpr int64_t kGatedRows = 64;
 int launch_gated_rows(const GatedArgs& a, hipStream_t st);

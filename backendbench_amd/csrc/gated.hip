@@ -1,5 +1,7 @@
 // The gated projection of a feed-forward block: h = act(x Wg^T) * (x Wu^T), W = [Wg; Wu] of 2F rows, and the
 // elementwise part of its backward pass.
+#include <string.h>
+
 #include "gated.h"
 #include "elementwise.h"
 
@@ -136,11 +138,21 @@ extern "C" int mi355_gated_linear(const void* x, int64_t x_rs, const void* weigh
   MI355_REQUIRE((x_rs >= K || M == 1) && w_rs >= K, "mi355_gated_linear: rows overlap (strides %lld, %lld for K = %lld)", (long long)x_rs,
                 (long long)w_rs, (long long)K);
   const GatedArgs a{x, weight, h, pre, M == 1 ? K : x_rs, w_rs, M, F, K, act, dtype};
-  const bool half = dtype == MI355_BF16 || dtype == MI355_F16;
-  const bool rows16 = a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && aligned16(x) && aligned16(weight);
-  const bool fits = M < (1 << 30) && F < (1 << 29) && K < (1 << 30);
-  if (half && fits && M <= kGatedRows) return launch_gated_rows(a, static_cast<hipStream_t>(stream));
-  if (half && rows16 && fits && gated_x16_takes(a)) return launch_gated_x16(a, static_cast<hipStream_t>(stream));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if ((dtype == MI355_BF16 || dtype == MI355_F16) && M < (1 << 30) && F < (1 << 29) && K > 0 && K < (1 << 30)) {
+    const bool rows16 = a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && aligned16(x) && aligned16(weight);
+    const bool few = M <= kGatedRows, t128 = rows16 && K % 64 == 0, t256 = rows16 && gated_x16_takes(a);
+    const char* form = knobs().gated_form;  // a test and measurement knob: one form, where it applies
+    if (form[0] != 0) {
+      if (few && (strcmp(form, "rows") == 0 || strcmp(form, "direct") == 0)) return launch_gated_rows(a, st);
+      if (t128 && strcmp(form, "tile128") == 0) return launch_gated_small2(a, st);
+      if (t256 && strcmp(form, "tile256") == 0) return launch_gated_x16(a, st);
+    }
+    const int64_t tiles = ((M + 127) / 128) * ((F + 63) / 64);  // of 128 rows by 64 features
+    if (few && (M <= 32 || !t128)) return launch_gated_rows(a, st);
+    if (t128 && (tiles <= kNumCU || !t256)) return launch_gated_small2(a, st);
+    if (t256) return launch_gated_x16(a, st);
+  }
   return set_error(MI355_ERR_UNSUPPORTED, "mi355_gated_linear: no single kernel for M=%lld F=%lld K=%lld %s", (long long)M, (long long)F,
                    (long long)K, dtype_name(dtype));
 }

@@ -1,6 +1,8 @@
 // The gated projection for few rows (decoding: 1 .. 64 tokens), bf16 / f16: the weight is read once and its stream is the
 // bound (4 F K bytes); v_mfma_f32_16x16x32 with the weight rows as the first operand, the waves of a workgroup share K and
 // add their accumulators in LDS at the end.  Two forms: through LDS for aligned rows, straight into registers for the rest.
+#include <string.h>
+
 #include "gated.h"
 #include "gemm_shared.h"
 
@@ -335,7 +337,7 @@ template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t 
     hipLaunchKernelGGL((gated_rows_kernel<T, MB, 1, W, S>), dim3((unsigned)((a.F + 15) / 16)), dim3(64 * W), 0, st, a);
     return check_launch("mi355_gated_linear");
   };
-  if (a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && a.K % 8 == 0 && aligned16(a.x) && aligned16(a.w)) {
+  if (strcmp(knobs().gated_form, "direct") != 0 && a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && a.K % 8 == 0 && aligned16(a.x) && aligned16(a.w)) {
     if (a.M <= 16) return lds(One(), One());
     if (a.M <= 32) return lds(Two(), Two());
     return lds(Four(), Two());

@@ -28,6 +28,7 @@
 
 #include "common.h"
 #include <atomic>
+#include "gated.h"
 #include "gemm_shared.h"
 
 namespace mi355 {
@@ -1552,24 +1553,88 @@ __global__ __launch_bounds__(256) void gemm_mfma_small_kernel(GemmArgs g) {
   }
 }
 
+// Epilogue of the gated projection on 32x32 blocks: a wave's 64 rows by 32 features, gate in acc[i][0], up in acc[i][1] (the
+// layout of store_tile_result), through the wave's slice of the idle ring, the left 64 bytes of 128-byte slab rows.
+struct GatedStore32 {
+  void* h;    // [M][F]
+  void* pre;  // [M][2F] or null
+  int act, vec;  // vec: rows of h and pre start on 16-byte boundaries
+
+  template <typename T>
+  __device__ __forceinline__ void store(const GemmArgs& g, const f32x16 (&acc)[2][2], unsigned char* lds, int wave, int lane, int m0, int f0) const {
+    const int fr = lane & 31, fg = lane >> 5;
+    unsigned char* slab = lds + wave * (64 * 128);
+    auto rows_out = [&](auto value, T* D, int64_t ld) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = i * 32 + fr;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          VecN4<T> r;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r.v[e] = static_cast<T>(value(i, q * 4 + e));
+          *reinterpret_cast<VecN4<T>*>(slab + row * 128 + ((q ^ ((row >> 1) & 7)) << 4) + fg * 8) = r;
+        }
+      }
+      // same wave wrote and reads: LDS operations of a wave complete in order
+      if (vec) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int unit = t * kWave + lane;  // 256 units of 16 bytes, 4 per row
+          const int row = unit >> 2, s = unit & 3;
+          const u32x4 v = *reinterpret_cast<const u32x4*>(slab + row * 128 + ((s ^ ((row >> 1) & 7)) << 4));
+          const int m = m0 + row, f = f0 + s * 8;
+          if (m < g.M && f < g.N) *reinterpret_cast<u32x4*>(D + (int64_t)m * ld + f) = v;
+        }
+      } else {
+        const int rows = g.M - m0 < 64 ? g.M - m0 : 64, cols = g.N - f0 < 32 ? g.N - f0 : 32;
+        store_slab_rows_shifted<T, 64>(slab, D, ld, m0, rows, f0, cols, lane);
+      }
+    };
+    if (pre != nullptr) {
+      T* P = static_cast<T*>(pre);
+      rows_out([&](int i, int r) __attribute__((always_inline)) { return acc[i][0][r]; }, P, 2 * (int64_t)g.N);
+      rows_out([&](int i, int r) __attribute__((always_inline)) { return acc[i][1][r]; }, P + g.N, 2 * (int64_t)g.N);
+    }
+    auto hidden = [&](auto ACT_) __attribute__((always_inline)) {
+      rows_out([&](int i, int r) __attribute__((always_inline)) {
+        const float gv = acc[i][0][r];
+        return gv * gate_q<decltype(ACT_)::value, GateHalf>(gv) * acc[i][1][r];
+      }, static_cast<T*>(h), g.N);
+    };
+    if (act == MI355_SILU) hidden(std::integral_constant<int, MI355_SILU>{});
+    else if (act == MI355_GELU) hidden(std::integral_constant<int, MI355_GELU>{});
+    else hidden(std::integral_constant<int, MI355_GELU_TANH>{});
+  }
+};
+
 // The 128x128 tile for launches with at most one workgroup per CU: nothing else hides a
 // workgroup's barrier, LDS and fill latencies there, so it owns the whole 160 KB of LDS (a ring of
 // five 64-k pairs, every request a whole 128-byte line), works in 64-k steps (16 MFMAs per wave
 // between barriers instead of 8) and reads its fragments a step ahead.
-template <typename T, bool B_NN, int SPLIT, bool A_T>
-__global__ __launch_bounds__(256) void gemm_mfma_small2_kernel(GemmArgs g) {
+//
+// GATE (any type but void): b is a gated projection's weight, [gate; up] of g.N rows each, K-contiguous, and the tile is 128
+// rows by 64 features: a wave's first 32-column block holds gate columns, its second the up columns of the same
+// features, which meet in one lane's accumulators; the epilogue is GATE's.
+template <typename T, bool B_NN, int SPLIT, bool A_T, typename GATE = void>
+__device__ __forceinline__ void small2_tile(const GemmArgs& g, unsigned char* lds, [[maybe_unused]] const GATE* gate = nullptr) {
+  constexpr bool GATED = !std::is_same<GATE, void>::value;
+  static_assert(!GATED || (!B_NN && SPLIT == 0 && !A_T), "the gated projection's form");
   constexpr int S = 5;  // ring depth in 64-k pairs
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   using frag_t = typename Mfma<T>::frag;
   const int tid = threadIdx.x, lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int wm = wave >> 1, wn = wave & 1;
   int tm, tn;
   tile_coords(g, tm, tn);
-  const int bm = tm * SBM, bn = tn * SBN;
+  const int bm = tm * SBM, bn = tn * (GATED ? SBN / 2 : SBN);
   const int kbeg = SPLIT ? (int)blockIdx.y * g.ksplit : 0;
   const int kend = SPLIT ? (kbeg + g.ksplit < g.K ? kbeg + g.ksplit : g.K) : g.K;
-  if ((int)blockIdx.x >= g.tiles_m * g.tiles_n) return warm_operands<T, A_T, B_NN>(g, kbeg, kend);
+  if ((int)blockIdx.x >= g.tiles_m * g.tiles_n) {
+    GemmArgs w = g;
+    if constexpr (GATED) w.N = 2 * g.N;
+    return warm_operands<T, A_T, B_NN>(w, kbeg, kend);
+  }
   const T* A = static_cast<const T*>(g.a) + (A_T ? (int64_t)kbeg * g.lda : (int64_t)kbeg);
   const T* B = static_cast<const T*>(g.b) + (B_NN ? (int64_t)kbeg * g.ldb : (int64_t)kbeg);
   const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
@@ -1597,7 +1662,11 @@ __global__ __launch_bounds__(256) void gemm_mfma_small2_kernel(GemmArgs g) {
       gr = gr < g.M ? gr : g.M - 1;
       a_src[i] = A + (int64_t)gr * g.lda + c * 8;
     }
-    if constexpr (!B_NN) {
+    if constexpr (GATED) {  // panel row r: column block (r / 32) % 2 (gate, up) of wave column r / 64
+      int gn = bn + (r >> 6) * 32 + (r & 31);
+      gn = gn < g.N ? gn : g.N - 1;
+      b_src[i] = B + ((int64_t)((r >> 5) & 1) * g.N + gn) * g.ldb + c * 8;
+    } else if constexpr (!B_NN) {
       int gn = bn + r;
       gn = gn < g.N ? gn : g.N - 1;
       b_src[i] = B + (int64_t)gn * g.ldb + c * 8;
@@ -1777,7 +1846,9 @@ __global__ __launch_bounds__(256) void gemm_mfma_small2_kernel(GemmArgs g) {
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (nothing is in flight: the last steps issue no fills)
 
-  if constexpr (SPLIT == 1) {
+  if constexpr (GATED) {
+    gate->template store<T>(g, acc, lds, wave, lane, bm + wm * 64, bn + wn * 32);
+  } else if constexpr (SPLIT == 1) {
     store_partial_tile<2>(g, acc, lane, bm + wm * 64, bn + wn * 64);
   } else {
     if constexpr (SPLIT == 2) {  // the parts meet inside this launch: the last one sums and stores
@@ -1786,6 +1857,46 @@ __global__ __launch_bounds__(256) void gemm_mfma_small2_kernel(GemmArgs g) {
     }
     store_tile_result<T, 2>(g, acc, lds, wave, lane, bm + wm * 64, bn + wn * 64);
   }
+}
+
+template <typename T, bool B_NN, int SPLIT, bool A_T>
+__global__ __launch_bounds__(256) void gemm_mfma_small2_kernel(GemmArgs g) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  small2_tile<T, B_NN, SPLIT, A_T>(g, lds);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void gated_small2_kernel(GemmArgs g, GatedStore32 out) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  small2_tile<T, false, 0, false, GatedStore32>(g, lds, &out);
+}
+
+// The gated projection on the deep-ring 128x128 tile (128 rows by 64 features): the caller has checked K % 64 == 0 and
+// 16-byte aligned rows.  CUs without a tile warm the last-level cache with the operands when the K loop is long enough.
+template <typename T> static int run_gated_small2(const GatedArgs& a, hipStream_t st) {
+  GemmArgs g{};
+  g.a = a.x;
+  g.b = a.w;
+  g.out = a.h;
+  g.lda = a.x_rs;
+  g.ldb = a.w_rs;
+  g.M = (int32_t)a.M;
+  g.N = (int32_t)a.F;
+  g.K = (int32_t)a.K;
+  g.tiles_m = (int32_t)((a.M + SBM - 1) / SBM);
+  g.tiles_n = (int32_t)((a.F + SBN / 2 - 1) / (SBN / 2));
+  const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n, idle = kNumCU - tiles;
+  const int64_t warm = idle >= 16 && a.K >= 1024 ? (idle < 32 ? idle : 32) : 0;
+  const GatedStore32 out{a.h, a.pre, a.act, a.F % 8 == 0 && aligned16(a.h) && aligned16(a.pre)};
+  const auto kern = gated_small2_kernel<T>;
+  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kSmall2Lds);
+  if (e != hipSuccess) return set_error(MI355_ERR_LAUNCH, "mi355_gated_linear: cannot reserve %d bytes of LDS: %s", kSmall2Lds, hipGetErrorString(e));
+  hipLaunchKernelGGL(kern, dim3((unsigned)(tiles + warm)), dim3(256), kSmall2Lds, st, g, out);
+  return check_launch("mi355_gated_linear");
+}
+
+int launch_gated_small2(const GatedArgs& a, hipStream_t st) {
+  return a.dtype == MI355_BF16 ? run_gated_small2<bf16_t>(a, st) : run_gated_small2<f16_t>(a, st);
 }
 
 // The deep-ring 128x128 kernel with the fills taken out of the computing waves' instruction streams: eight

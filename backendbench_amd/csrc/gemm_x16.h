@@ -409,8 +409,7 @@ template <typename T, bool B_NN, int NPQ, bool PERSIST = false, bool SPLITK = fa
 __device__ __forceinline__ void x16_tile(const GemmArgs& g, unsigned char* lds, int bm, int bn, const X16Split& sk = X16Split{},
                                          [[maybe_unused]] const GATE* gate = nullptr) {
   constexpr bool GATED = !std::is_same<GATE, void>::value;
-  static_assert(!GATED || (!B_NN && NPQ == 4 && !SPLITK), "the gated projection's form");
-  constexpr int TN = GATED ? 128 : BN;  // columns of the result per tile
+  static_assert(!GATED || (!B_NN && NPQ == 4 && !PERSIST && !SPLITK), "the gated projection's form");
   static_assert(NPQ == 3 || NPQ == 4, "wave tile is 128 x 32 NPQ");
   static_assert(!PERSIST || NPQ == 4, "the persistent form walks 256 x 256 tiles");
   using frag_t = typename Mfma16<T>::frag;
@@ -457,7 +456,7 @@ __device__ __forceinline__ void x16_tile(const GemmArgs& g, unsigned char* lds, 
   // at the edge (M, N >= 256): every tile stays whole, and the rows / columns it shares with its neighbour are
   // computed - from the same k sequence - and stored twice with the same values.
   auto row0 = [&](int tm) { const int m = tm * BM; return m + BM <= g.M ? m : g.M - BM; };
-  auto col0 = [&](int tn) { const int n = tn * TN; return n + TN <= g.N ? n : g.N - TN; };
+  auto col0 = [&](int tn) { const int n = tn * BN; return n + BN <= g.N ? n : g.N - BN; };
   const unsigned char* a_base = a_start(PERSIST ? row0(ptm) : bm);  // of the tile being computed
   const unsigned char* b_base = b_start(PERSIST ? col0(ptn) : bn);
   const int64_t a_step = 128;                                   // bytes per 64-k stage
@@ -641,7 +640,6 @@ __device__ __forceinline__ void x16_tile(const GemmArgs& g, unsigned char* lds, 
     }
 #else
     if constexpr (WAIT == 56) asm volatile("s_waitcnt vmcnt(56)" ::: "memory");
-    if constexpr (WAIT == 40) asm volatile("s_waitcnt vmcnt(40)" ::: "memory");
     if constexpr (WAIT == 24 && !(MI355_X16_ABLATE & 8)) asm volatile("s_waitcnt vmcnt(24)" ::: "memory");
     if constexpr (WAIT == 16) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
     if constexpr (WAIT == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
@@ -651,6 +649,7 @@ __device__ __forceinline__ void x16_tile(const GemmArgs& g, unsigned char* lds, 
     rd = bump(rd);
     fl = bump(fl);
   };
+  using W56 = std::integral_constant<int, 56>;
   using W24 = std::integral_constant<int, 24>;
   using W16 = std::integral_constant<int, 16>;
   using W8 = std::integral_constant<int, 8>;
@@ -710,10 +709,9 @@ __device__ __forceinline__ void x16_tile(const GemmArgs& g, unsigned char* lds, 
       const unsigned char* fb = b_base + 2 * b_step;
       // First four half-stages (np >= 12): pairs 2 .. 4 were requested before the previous tile's 32
       // stores per lane, pair 5 behind them - only the wait for pair 5 has to see the stores out.
-      using WS = std::integral_constant<int, 24 + (GATED ? 16 : 32)>;  // the gated epilogue issues 16 stores at least
-      half_stage(I0{}, Yes{}, Yes{}, WS{}, Yes{}, fa, fb);
-      half_stage(I1{}, Yes{}, Yes{}, WS{}, Yes{}, fa + a_step, fb + b_step);
-      half_stage(I2{}, Yes{}, Yes{}, WS{}, Yes{}, fa + a_step, fb + b_step);
+      half_stage(I0{}, Yes{}, Yes{}, W56{}, Yes{}, fa, fb);
+      half_stage(I1{}, Yes{}, Yes{}, W56{}, Yes{}, fa + a_step, fb + b_step);
+      half_stage(I2{}, Yes{}, Yes{}, W56{}, Yes{}, fa + a_step, fb + b_step);
       half_stage(I3{}, Yes{}, Yes{}, W24{}, Yes{}, fa + 2 * a_step, fb + 2 * b_step);
       fa += 2 * a_step;
       fb += 2 * b_step;
@@ -737,8 +735,7 @@ __device__ __forceinline__ void x16_tile(const GemmArgs& g, unsigned char* lds, 
       // the last MFMA's result is read by VALU moves next; the slot of the pair just read (`fl`) is free
       // until the next half-stage requests into it
       asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
-      if constexpr (GATED) gate->template store<T, 2>(g, acc, lds + fl, wave, lane, row0(ptm) + wm * 128, col0(ptn) + wn * 64);
-      else store_tile_result16<T, NPQ, 2>(g, acc, lds + fl, wave, lane, row0(ptm) + wm * 128, col0(ptn) + wn * 128);
+      store_tile_result16<T, NPQ, 2>(g, acc, lds + fl, wave, lane, row0(ptm) + wm * 128, col0(ptn) + wn * 128);
       __syncthreads();  // every wave is done with its slab before anyone requests into the slot
       if (!has_next) break;
       pid = npid; ptm = ntm; ptn = ntn;
@@ -862,7 +859,7 @@ __device__ __forceinline__ void x16_tile(const GemmArgs& g, unsigned char* lds, 
   }
   if (!(MI355_X16_ABLATE & 32) || g.alpha == 12345.f) {
     if constexpr (GATED) {
-      gate->template store<T, 1>(g, acc, lds, wave, lane, bm + wm * 128, bn + wn * 64);
+      gate->template store<T>(g, acc, lds, wave, lane, bm + wm * 128, bn + wn * 64);
     } else if constexpr (NPQ == 4) {
       if (g.out_rows) store_tile_rows16<T>(g, acc, lds, wave, lane, bm, bn);
       else store_tile_result16<T, NPQ>(g, acc, lds, wave, lane, bm + wm * 128, bn + wn * WCOLS);

@@ -253,6 +253,31 @@ def test_gated_linear(M, K, F, dtype):
     gated_backward_check(got, dh, x, w, pre, act, f"{M}x{K}x{F} {act}")
 
 
+@pytest.fixture
+def gated_form():
+    yield lambda value: _lib.set_knob("gated_form", value)
+    _lib.set_knob("gated_form", None)
+
+
+@pytest.mark.parametrize("form,M,K,F", [
+    ("rows", 1, 2048, 40), ("rows", 16, 1016, 24), ("rows", 17, 2056, 23), ("rows", 64, 4104, 129), ("rows", 33, 8, 1), ("rows", 5, 5120, 8),
+    ("direct", 1, 2048, 40), ("direct", 40, 1000, 129), ("direct", 20, 77, 9),
+    ("tile128", 1, 64, 1), ("tile128", 130, 128, 70), ("tile128", 64, 192, 64), ("tile128", 300, 256, 129), ("tile128", 257, 448, 200),
+    ("tile128", 128, 1024, 336),
+    ("tile256", 1, 256, 1), ("tile256", 300, 384, 129), ("tile256", 257, 640, 128), ("tile256", 512, 1024, 264),
+    ("tile256", 1000, 640, 4104)])
+@pytest.mark.parametrize("dtype", HALF)
+def test_gated_linear_forms(gated_form, form, M, K, F, dtype):
+    """Every kernel form on shapes of the test's choosing: ragged and single tiles, short K loops, with and without pre."""
+    g = generator(M + F)
+    x, w = randn(g, M, K, dtype=dtype), randn(g, 2 * F, K, dtype=dtype, scale=K ** -0.5)
+    act = ["silu", "gelu", "gelu_tanh"][F % 3]
+    gated_form(form)
+    h, pre = ops.gated_linear(x, w, act, save_pre=True)
+    gated_forward_check(h, pre, x, w, act, f"{form} {M}x{K}x{F} {act}")
+    assert torch.equal(ops.gated_linear(x, w, act), h)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
 def test_gated_linear_far_gates(act, dtype):
