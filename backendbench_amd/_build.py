@@ -25,6 +25,7 @@ SOURCES = [
     "layernorm.hip",
     "layernorm_bwd.hip",
     "gated.hip",
+    "gated_backward.hip",
     "gated_x16.hip",
     "gated_rows.hip",
     "dropout.hip",

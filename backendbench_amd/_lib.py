@@ -121,7 +121,12 @@ TRAIN_SIGNATURES = {
         [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p],
     ),
     "mi355_gated_act": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p]),
-    "mi355_gated_act_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p]),
+    "mi355_gated_linear_backward_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
+    "mi355_gated_linear_backward": (
+        c_int,
+        [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int,
+         c_void_p, c_int64, c_void_p],
+    ),
     "mi355_dropout_add": (
         c_int,
         [c_void_p, c_void_p, c_int, c_double, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p],

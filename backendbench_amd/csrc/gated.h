@@ -1,5 +1,7 @@
 // The activations of the gated projection and their derivatives.
 #pragma once
+#include <type_traits>
+
 #include "../../include/mi355_train.h"
 #include "common.h"
 
@@ -58,6 +60,16 @@ template <int ACT, typename A, typename F> __device__ __forceinline__ F gate_gra
 }
 // The arithmetic for results of type T.
 template <typename T> using GateMath = std::conditional_t<sizeof(T) == 2, GateHalf, typename OpMath<T>::type>;
+
+// body(ACT) with an integral constant.
+template <typename Body> static int dispatch_act(int act, const char* name, Body body) {
+  switch (act) {
+    case MI355_SILU: body(std::integral_constant<int, MI355_SILU>()); return MI355_OK;
+    case MI355_GELU: body(std::integral_constant<int, MI355_GELU>()); return MI355_OK;
+    case MI355_GELU_TANH: body(std::integral_constant<int, MI355_GELU_TANH>()); return MI355_OK;
+    default: return set_error(MI355_ERR_INVALID, "%s: unknown activation %d", name, act);
+  }
+}
 
 // One gated projection: x [M][K], weight [2F][K] (gate rows, then up rows), both K-contiguous; h [M][F]; pre [M][2F] or null.
 struct GatedArgs {

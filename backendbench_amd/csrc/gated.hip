@@ -1,5 +1,5 @@
-// The gated projection of a feed-forward block: h = act(x Wg^T) * (x Wu^T), W = [Wg; Wu] of 2F rows, and the
-// elementwise part of its backward pass.
+// The gated projection of a feed-forward block, h = act(x Wg^T) * (x Wu^T), W = [Wg; Wu] of 2F rows: which kernel takes a
+// call, and the activation as a kernel of its own behind a product (fp32, fp64, and layouts no single kernel takes).
 #include <string.h>
 
 #include "gated.h"
@@ -34,37 +34,6 @@ __global__ __launch_bounds__(256) void gated_act_kernel(const P* __restrict__ pr
   }
 }
 
-template <typename T, int ACT, int V>
-__global__ __launch_bounds__(256) void gated_act_backward_kernel(const T* __restrict__ dh, const T* __restrict__ pre,
-                                                                T* __restrict__ dpre, int64_t items, int64_t per_row, int64_t F) {
-  using A = typename OpMath<T>::type;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
-    const int64_t m = items < (int64_t(1) << 32) ? (uint32_t)i / (uint32_t)per_row : i / per_row;
-    const int64_t f = (i - m * per_row) * V;
-    const VecN<T, V> g = ld_nt<T, V>(pre + m * 2 * F + f), u = ld_nt<T, V>(pre + m * 2 * F + F + f), d = ld_nt<T, V>(dh + m * F + f);
-    VecN<T, V> dg, du;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const A ga = static_cast<A>(g.v[j]), ua = static_cast<A>(u.v[j]), da = static_cast<A>(d.v[j]);
-      const A q = gate_q<ACT, GateMath<T>>(ga);
-      dg.v[j] = static_cast<T>(da * ua * gate_grad<ACT, GateMath<T>>(ga, q));
-      du.v[j] = static_cast<T>(da * (ga * q));
-    }
-    st<T, V>(dpre + m * 2 * F + f, dg);
-    st<T, V>(dpre + m * 2 * F + F + f, du);
-  }
-}
-
-// body(ACT) with an integral constant.
-template <typename Body> static int dispatch_act(int act, const char* name, Body body) {
-  switch (act) {
-    case MI355_SILU: body(std::integral_constant<int, MI355_SILU>()); return MI355_OK;
-    case MI355_GELU: body(std::integral_constant<int, MI355_GELU>()); return MI355_OK;
-    case MI355_GELU_TANH: body(std::integral_constant<int, MI355_GELU_TANH>()); return MI355_OK;
-    default: return set_error(MI355_ERR_INVALID, "%s: unknown activation %d", name, act);
-  }
-}
-
 template <typename T, typename P>
 static int run_gated_act(const void* pre, void* h, void* pre_out, int64_t M, int64_t F, int act, hipStream_t st) {
   constexpr int V = 16 / sizeof(P);  // whole 16-byte reads
@@ -84,23 +53,6 @@ static int run_gated_act(const void* pre, void* h, void* pre_out, int64_t M, int
   return rc != MI355_OK ? rc : check_launch("mi355_gated_act");
 }
 
-template <typename T>
-static int run_gated_act_backward(const void* dh, const void* pre, void* dpre, int64_t M, int64_t F, int act, hipStream_t st) {
-  constexpr int V = 16 / sizeof(T);
-  const bool vec = F % V == 0 && aligned16(pre) && aligned16(dh) && aligned16(dpre);
-  const int rc = dispatch_act(act, "mi355_gated_act_backward", [&](auto a) {
-    constexpr int ACT = decltype(a)::value;
-    auto go = [&](auto v) {
-      constexpr int VV = decltype(v)::value;
-      const int64_t items = M * (F / VV);
-      hipLaunchKernelGGL((gated_act_backward_kernel<T, ACT, VV>), dim3((unsigned)grid_for(items, 256, 1 << 20)), dim3(256), 0, st,
-                         static_cast<const T*>(dh), static_cast<const T*>(pre), static_cast<T*>(dpre), items, F / VV, F);
-    };
-    vec ? go(std::integral_constant<int, V>()) : go(std::integral_constant<int, 1>());
-  });
-  return rc != MI355_OK ? rc : check_launch("mi355_gated_act_backward");
-}
-
 }  // namespace mi355
 
 using namespace mi355;
@@ -117,16 +69,6 @@ extern "C" int mi355_gated_act(const void* pre, int pre_dtype, void* h, void* pr
   if (pre_dtype != dtype)
     return set_error(MI355_ERR_UNSUPPORTED, "mi355_gated_act: no kernel for %s from %s", dtype_name(dtype), dtype_name(pre_dtype));
   MI355_DISPATCH_FLOAT(dtype, "mi355_gated_act", return run_gated_act<T, T>(pre, h, pre_out, M, F, act, st));
-}
-
-extern "C" int mi355_gated_act_backward(const void* dh, const void* pre, void* dpre, int dtype, int64_t M, int64_t F, int act,
-                                        void* stream) {
-  MI355_REQUIRE(M >= 0 && F >= 0, "mi355_gated_act_backward: negative extent");
-  MI355_REQUIRE(act >= MI355_SILU && act <= MI355_GELU_TANH, "mi355_gated_act_backward: unknown activation %d", act);
-  if (M == 0 || F == 0) return MI355_OK;
-  MI355_REQUIRE(dh != nullptr && pre != nullptr && dpre != nullptr, "mi355_gated_act_backward: NULL data pointer");
-  MI355_DISPATCH_FLOAT(dtype, "mi355_gated_act_backward",
-                       return run_gated_act_backward<T>(dh, pre, dpre, M, F, act, static_cast<hipStream_t>(stream)));
 }
 
 extern "C" int mi355_gated_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, void* h, void* pre, int64_t M, int64_t F,

@@ -204,12 +204,16 @@ def _gated_linear_backward(grad_out, input, weight, pre, activation, mask):
     dtype, device = input.dtype, input.device
     if M == 0 or F == 0 or K == 0 or not any(mask):
         return (torch.zeros_like(input) if mask[0] else None), (torch.zeros_like(weight) if mask[1] else None)
-    dh, p, x = dense(grad_out), dense(pre), dense(input).view(M, K)
-    dpre = new_dense((M, 2 * F), dtype, device)
-    launch("mi355_gated_act_backward", dh.data_ptr(), p.data_ptr(), dpre.data_ptr(), _lib.dtype_code(dtype), M, F,
-           _ACTIVATIONS[activation])
-    dx = _gemm(dpre, weight, None, 1.0, 0.0).view(input.shape) if mask[0] else None
-    dw = _gemm(dpre.t(), x, None, 1.0, 0.0) if mask[1] else None
+    dh, p, x = dense(grad_out), dense(pre), dense(input)
+    w = weight if weight.stride(1) == 1 and weight.stride(0) >= K else dense(weight)
+    dx = new_dense(input.shape, dtype, device) if mask[0] else None
+    dw = new_dense(weight.shape, dtype, device) if mask[1] else None
+    code = _lib.dtype_code(dtype)
+    ws_bytes = _lib.load().mi355_gated_linear_backward_workspace_bytes(M, F, K, code)
+    ws = new_dense((ws_bytes,), torch.uint8, device)
+    launch("mi355_gated_linear_backward", dh.data_ptr(), x.data_ptr(), K, w.data_ptr(), w.stride(0), p.data_ptr(),
+           dx.data_ptr() if mask[0] else None, dw.data_ptr() if mask[1] else None, M, F, K, _ACTIVATIONS[activation], code,
+           ws.data_ptr(), ws_bytes)
     return dx, dw
 
 

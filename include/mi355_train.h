@@ -49,9 +49,15 @@ int mi355_gated_linear(const void* x, int64_t x_rs, const void* weight, int64_t 
 int mi355_gated_act(const void* pre, int pre_dtype, void* h, void* pre_out, int dtype, int64_t M, int64_t F, int act,
                     void* stream);
 
-/* dpre[m][f] = dh * up * act'(gate), dpre[m][F + f] = dh * act(gate) with gate = pre[m][f], up = pre[m][F + f]; all
- * dense and of `dtype`; computed in fp32 (fp64 for f64). */
-int mi355_gated_act_backward(const void* dh, const void* pre, void* dpre, int dtype, int64_t M, int64_t F, int act, void* stream);
+/* Its gradients: dpre = [dh * up * act'(gate) | dh * act(gate)] with gate = pre[m][f], up = pre[m][F + f], rounded once to
+ * `dtype` (f32, f16, bf16, f64), then dx [M][K] = dpre W and dweight [2F][K] = dpre^T x, accumulated in fp32 (fp64).  dh
+ * [M][F], pre [M][2F], dx and dweight are dense; x and weight have rows x_rs and w_rs apart.  dx or dweight may be NULL.
+ * The workspace (16-byte aligned, contents undefined before and after; not shared by calls that may overlap in time)
+ * holds dpre and the products' scratch: mi355_gated_linear_backward_workspace_bytes() always suffices. */
+int64_t mi355_gated_linear_backward_workspace_bytes(int64_t M, int64_t F, int64_t K, int dtype);
+int mi355_gated_linear_backward(const void* dh, const void* x, int64_t x_rs, const void* weight, int64_t w_rs, const void* pre,
+                                void* dx, void* dweight, int64_t M, int64_t F, int64_t K, int act, int dtype,
+                                void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- dropout with a residual ------------------------------------------------------- */
 

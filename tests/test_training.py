@@ -148,10 +148,28 @@ def test_c_entry_points_check_their_arguments():
     refused(act(p, _lib.F16, p, None, _lib.F32, 4, 8, 0, None), b"no kernel")
     refused(act(p, _lib.I32, p, None, _lib.I32, 4, 8, 0, None), b"unsupported")
     refused(act(p, _lib.F32, p, None, _lib.F32, -4, 8, 0, None), b"negative")
-    back = lib.mi355_gated_act_backward
-    refused(back(p, p, None, _lib.F32, 4, 8, 0, None), b"NULL")
-    refused(back(p, p, p, _lib.F32, 4, 8, -1, None), b"activation")
-    refused(back(p, p, p, _lib.U8, 4, 8, 0, None), b"unsupported")
+    fwd = lib.mi355_gated_linear
+    refused(fwd(p, 64, p, 64, p, None, 4, 8, 64, 3, _lib.BF16, None), b"activation")
+    refused(fwd(None, 64, p, 64, p, None, 4, 8, 64, 0, _lib.BF16, None), b"NULL")
+    refused(fwd(p, 63, p, 64, p, None, 4, 8, 64, 0, _lib.BF16, None), b"overlap")
+    refused(fwd(p, 64, p, 0, p, None, 4, 8, 64, 0, _lib.BF16, None), b"overlap")
+    refused(fwd(p, 64, p, 64, p, None, 4, -8, 64, 0, _lib.BF16, None), b"negative")
+    for rows, K, dtype in ((4, 64, _lib.F32), (4, 64, _lib.F64), (4, 64, _lib.I8), (65, 63, _lib.BF16), (65, 72, _lib.F16), (4, 0, _lib.BF16)):
+        assert fwd(p, K, p, K, p, None, rows, 8, K, 0, dtype, None) == -2     # unsupported, nothing launched
+    assert fwd(None, 64, None, 64, None, None, 0, 8, 64, 0, _lib.BF16, None) == 0
+    back, size = lib.mi355_gated_linear_backward, lib.mi355_gated_linear_backward_workspace_bytes
+    need = size(4, 8, 64, _lib.F32)
+    assert need > 0 and size(0, 8, 64, _lib.F32) == 0 and size(4, 8, 64, _lib.U8) == 0
+    refused(back(p, p, 64, p, 64, p, p, p, 4, 8, 64, -1, _lib.F32, p, need, None), b"activation")
+    refused(back(p, p, 64, p, 64, None, p, p, 4, 8, 64, 0, _lib.F32, p, need, None), b"NULL")
+    refused(back(p, p, 60, p, 64, p, p, p, 4, 8, 64, 0, _lib.F32, p, need, None), b"overlap")
+    refused(back(p, p, 64, p, 64, p, p, p, 4, 8, 64, 0, _lib.F32, p, 16, None), b"workspace")
+    refused(back(p, p, 64, p, 64, p, p, p, 4, 8, 64, 0, _lib.F32, p + 8, need, None), b"workspace")
+    refused(back(p, p, 64, p, 64, p, p, p, 4, 8, 64, 0, _lib.F32, None, need, None), b"workspace")
+    refused(back(p, p, 64, p, 64, p, p, p, 4, 8, 64, 0, _lib.U8, p, need, None), b"unsupported")
+    refused(back(p, p, 64, p, 64, p, p, p, 0, 8, 64, 0, _lib.F32, p, need, None), b"empty")
+    refused(back(p, p, 64, p, 64, p, p, p, 4, 8, -64, 0, _lib.F32, p, need, None), b"negative")
+    assert back(None, None, 64, None, 64, None, None, None, 4, 8, 64, 0, _lib.F32, None, 0, None) == 0
     drop = lib.mi355_dropout_add
     refused(drop(p, None, _lib.F32, 1.5, None, 0, 0, p, 4, None), b"[0, 1]")
     refused(drop(p, None, _lib.F32, float("nan"), None, 0, 0, p, 4, None), b"[0, 1]")
@@ -216,3 +234,17 @@ def test_gated_formula_against_differences(act):
     dpre = ref.gated_pre_backward(dh, ref.gated_linear(x, w, act)[0][1], act)
     assert torch.allclose(dpre @ w, differences(lambda t: loss(t, w), x), rtol=1e-6, atol=1e-7)
     assert torch.allclose(dpre.t() @ x, differences(lambda t: loss(x, t), w), rtol=1e-6, atol=1e-7)
+
+
+def test_gated_backward_workspace_covers_every_alignment():
+    """The size a caller asks for covers what any alignment of the operands takes (a call with less is refused)."""
+    lib, p = _lib.load(), 1 << 20
+    for M, F, K, dtype in ((64, 64, 64, _lib.BF16), (65, 33, 77, _lib.F16), (300, 1000, 768, _lib.BF16), (5, 3, 7, _lib.F32), (7, 9, 11, _lib.F64)):
+        full = lib.mi355_gated_linear_backward_workspace_bytes(M, F, K, dtype)
+        es = 2 if dtype in (_lib.F16, _lib.BF16) else 4 if dtype == _lib.F32 else 8
+        assert full >= 2 * M * F * es and full % 256 == 0
+        for x_off, w_off in ((0, 0), (es, 0), (0, es), (es, es)):
+            for dx, dw in ((p, p), (p, None), (None, p)):
+                rc = lib.mi355_gated_linear_backward(p, p + x_off, K, p + w_off, K, p, dx, dw, M, F, K, 0, dtype, p, 0, None)
+                need = int(re.search(rb"workspace of (\d+) bytes", lib.mi355_last_error()).group(1))
+                assert rc == -1 and 0 < need <= full, (M, F, K, dtype, need, full)
