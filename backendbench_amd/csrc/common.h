@@ -2,6 +2,7 @@
 // access, wave64 reductions (DPP inside 16-lane rows, bpermute across rows), dimension
 // collapsing and the thread-local error string behind mi355_last_error().
 #pragma once
+#include <atomic>
 #include <type_traits>
 
 #include <hip/hip_runtime.h>
@@ -283,6 +284,18 @@ int check_tensor(const mi355_tensor* t, const char* op, const char* name);
 // If every tensor has identical strides that tile memory densely in some dim order
 // (a permuted-contiguous layout), the op is a flat 1-D pass over `numel` elements.
 bool same_dense_layout(const mi355_tensor* const* ts, int nt);
+
+// Lets `kern` take `bytes` of dynamic LDS on the current device; asked of the runtime once per kernel and device (`devices`:
+// one bit each, a static of the caller's).
+inline int allow_lds(const void* kern, int bytes, std::atomic<uint64_t>& devices, const char* what) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) dev = 64;
+  if (dev < 64 && (devices.load(std::memory_order_relaxed) >> dev & 1)) return MI355_OK;
+  const hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return set_error(MI355_ERR_LAUNCH, "%s: cannot reserve %d bytes of LDS: %s", what, bytes, hipGetErrorString(e));
+  if (dev < 64) devices.fetch_or(uint64_t(1) << dev, std::memory_order_relaxed);
+  return MI355_OK;
+}
 
 inline int grid_for(int64_t work_items, int per_block, int max_blocks) {
   int64_t b = (work_items + per_block - 1) / per_block;

@@ -77,9 +77,9 @@ extern "C" int mi355_gated_linear(const void* x, int64_t x_rs, const void* weigh
   MI355_REQUIRE(act >= MI355_SILU && act <= MI355_GELU_TANH, "mi355_gated_linear: unknown activation %d", act);
   if (M == 0 || F == 0) return MI355_OK;
   MI355_REQUIRE(x != nullptr && weight != nullptr && h != nullptr, "mi355_gated_linear: NULL data pointer");
-  MI355_REQUIRE((x_rs >= K || M == 1) && w_rs >= K, "mi355_gated_linear: rows overlap (strides %lld, %lld for K = %lld)", (long long)x_rs,
+  MI355_REQUIRE(x_rs >= K && w_rs >= K, "mi355_gated_linear: rows overlap (strides %lld, %lld for K = %lld)", (long long)x_rs,
                 (long long)w_rs, (long long)K);
-  const GatedArgs a{x, weight, h, pre, M == 1 ? K : x_rs, w_rs, M, F, K, act, dtype};
+  const GatedArgs a{x, weight, h, pre, x_rs, w_rs, M, F, K, act, dtype};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if ((dtype == MI355_BF16 || dtype == MI355_F16) && M < (1 << 30) && F < (1 << 29) && K > 0 && K < (1 << 30)) {
     const bool rows16 = a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && aligned16(x) && aligned16(weight);
@@ -90,9 +90,12 @@ extern "C" int mi355_gated_linear(const void* x, int64_t x_rs, const void* weigh
       if (t128 && strcmp(form, "tile128") == 0) return launch_gated_small2(a, st);
       if (t256 && strcmp(form, "tile256") == 0) return launch_gated_x16(a, st);
     }
+    // Measured ([M, 4096] x 2 * 11008 and [M, 2048] x 2 * 5504, us): rows against 128-row tiles 46.7 / 48.7 and 17.7 / 19 at 32
+    // rows, 60 / 48 and 23 / 19.4 at 48, 69 / 49.5 and 26.4 / 19.8 at 64; 128- against 256-row tiles 55 / 77 and 22 / 41 with 172
+    // and 86 of the former, 22.7 / 42 with 172, 78 / 79.5 and 42 / 43.5 with 344, 122 / 89 and 64 / 48 with 688.
     const int64_t tiles = ((M + 127) / 128) * ((F + 63) / 64);  // of 128 rows by 64 features
     if (few && (M <= 32 || !t128)) return launch_gated_rows(a, st);
-    if (t128 && (tiles <= kNumCU || !t256)) return launch_gated_small2(a, st);
+    if (t128 && tiles <= (t256 ? kNumCU : 2 * kNumCU)) return launch_gated_small2(a, st);
     if (t256) return launch_gated_x16(a, st);
   }
   return set_error(MI355_ERR_UNSUPPORTED, "mi355_gated_linear: no single kernel for M=%lld F=%lld K=%lld %s", (long long)M, (long long)F,

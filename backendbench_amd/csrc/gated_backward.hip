@@ -13,33 +13,61 @@ namespace mi355 {
 
 constexpr int kGbTile = 64;
 
-// Tiles of 64 rows by 64 features, 256 threads.  ROW: dpre [M][ld] (columns 2F .. ld - 1 become zeros); COL: its transpose
-// dpre_t [2F][ld_t] (columns M .. ld_t - 1 become zeros), through LDS.  VEC: F a multiple of the vector, aligned operands.
-template <typename T, int ACT, bool ROW, bool COL, bool VEC>
+// 16 bytes at an address that is only a multiple of an element's size.
+template <int B> struct GbAny;
+template <> struct GbAny<2> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct GbAny<4> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct GbAny<8> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(8))); };
+// The V = 16 / sizeof(T) elements from p on, of which `count` are there (the rest become zeros).
+template <typename T, int V = 16 / sizeof(T)> __device__ __forceinline__ VecN<T, V> gb_load(const T* p, int64_t count) {
+  VecN<T, V> v{};
+  if (count >= V) {
+    v = __builtin_bit_cast(decltype(v), __builtin_nontemporal_load(reinterpret_cast<const typename GbAny<sizeof(T)>::type*>(p)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < count) v.v[j] = p[j];
+  }
+  return v;
+}
+template <typename T, int V> __device__ __forceinline__ void gb_store(T* p, int64_t count, const VecN<T, V>& v) {
+  if (count >= V) {
+    *reinterpret_cast<typename GbAny<sizeof(T)>::type*>(p) = __builtin_bit_cast(u32x4, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < count) p[j] = v.v[j];
+  }
+}
+
+// Tiles of TM rows by 64 features, 256 threads: 64 rows, so that the transpose goes out in whole 128-byte lines (6.2 TB/s at
+// [4096, 2 * 11008] bf16, 102 us), or 16 where tiles of 64 would leave most CUs idle ([197, 2 * 1001] fp32: 64 tiles 15 us,
+// 256 tiles 6.5).  ROW: dpre [M][ld] (columns 2F .. ld - 1 become zeros); COL: its transpose dpre_t [2F][ld_t] (columns M ..
+// ld_t - 1 become zeros), through LDS.  Vector accesses at any alignment.
+template <typename T, int ACT, bool ROW, bool COL, int TM>
 __global__ __launch_bounds__(256) void gated_dpre_kernel(const T* __restrict__ dh, const T* __restrict__ pre, T* __restrict__ dpre, int64_t ld,
                                                         T* __restrict__ dpre_t, int64_t ld_t, int64_t M, int64_t F, int tiles_f) {
   using A = typename OpMath<T>::type;
-  constexpr int V = VEC ? 16 / sizeof(T) : 1;
-  constexpr int PER = kGbTile * kGbTile / V / 256;  // vectors per thread
-  constexpr int LD = kGbTile + 4 / sizeof(T);       // one bank further per feature
+  constexpr int V = 16 / sizeof(T);
+  constexpr int VECS = TM * kGbTile / V, PER = (VECS + 255) / 256;  // vectors of the tile, and per thread
+  constexpr int LD = TM + 4 / sizeof(T);            // one bank further per feature
   __shared__ T turned[COL ? 2 : 1][COL ? kGbTile : 1][COL ? LD : 1];
-  const int64_t m0 = (int64_t)(blockIdx.x / tiles_f) * kGbTile, f0 = (int64_t)(blockIdx.x % tiles_f) * kGbTile;
+  const int64_t m0 = (int64_t)(blockIdx.x / tiles_f) * TM, f0 = (int64_t)(blockIdx.x % tiles_f) * kGbTile;
   VecN<T, V> gv[PER], uv[PER], dv[PER];
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int e = (threadIdx.x + 256 * i) * V;
     const int64_t m = m0 + e / kGbTile, f = f0 + e % kGbTile;
-    gv[i] = uv[i] = dv[i] = VecN<T, V>{};
-    if (m < M && f < F) {
-      gv[i] = ld_nt<T, V>(pre + m * 2 * F + f);
-      uv[i] = ld_nt<T, V>(pre + m * 2 * F + F + f);
-      dv[i] = ld_nt<T, V>(dh + m * F + f);
-    }
+    const int64_t there = m < M && e < TM * kGbTile ? F - f : 0;
+    gv[i] = gb_load(pre + m * 2 * F + f, there);
+    uv[i] = gb_load(pre + m * 2 * F + F + f, there);
+    dv[i] = gb_load(dh + m * F + f, there);
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     const int e = (threadIdx.x + 256 * i) * V;
     const int64_t m = m0 + e / kGbTile, f = f0 + e % kGbTile;
+    if (e >= TM * kGbTile) break;
     VecN<T, V> dg, du;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -53,15 +81,14 @@ __global__ __launch_bounds__(256) void gated_dpre_kernel(const T* __restrict__ d
       }
     }
     if constexpr (ROW) {
-      if (m < M && f < F) {
-        st<T, V>(dpre + m * ld + f, dg);
-        st<T, V>(dpre + m * ld + F + f, du);
-      }
+      const int64_t there = m < M ? F - f : 0;
+      gb_store(dpre + m * ld + f, there, dg);
+      gb_store(dpre + m * ld + F + f, there, du);
     }
   }
   if constexpr (ROW) {
     if (f0 + kGbTile >= F && ld > 2 * F) {
-      for (int e = threadIdx.x; e < kGbTile * (int)(ld - 2 * F); e += 256) {
+      for (int e = threadIdx.x; e < TM * (int)(ld - 2 * F); e += 256) {
         const int64_t m = m0 + e / (int)(ld - 2 * F);
         if (m < M) dpre[m * ld + 2 * F + e % (int)(ld - 2 * F)] = static_cast<T>(0.f);
       }
@@ -71,9 +98,9 @@ __global__ __launch_bounds__(256) void gated_dpre_kernel(const T* __restrict__ d
     __syncthreads();
     constexpr int W = 16 / sizeof(T);  // ld_t is a multiple of it
 #pragma unroll
-    for (int i = 0; i < 2 * kGbTile * kGbTile / W / 256; ++i) {
+    for (int i = 0; i < 2 * TM * kGbTile / W / 256; ++i) {
       const int e = (threadIdx.x + 256 * i) * W;
-      const int which = e / (kGbTile * kGbTile), fl = e / kGbTile % kGbTile, ml = e % kGbTile;
+      const int which = e / (TM * kGbTile), fl = e / TM % kGbTile, ml = e % TM;
       if (f0 + fl >= F || m0 + ml >= ld_t) continue;
       VecN<T, W> v;
 #pragma unroll
@@ -90,16 +117,29 @@ __global__ __launch_bounds__(256) void turn_pad_kernel(const B* __restrict__ src
   constexpr int LD = kGbTile + 4 / sizeof(B);
   __shared__ B tile[kGbTile][LD];
   const int64_t r0 = (int64_t)(blockIdx.x / tiles_c) * kGbTile, c0 = (int64_t)(blockIdx.x % tiles_c) * kGbTile;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < kGbTile * kGbTile; e += 256) {
+  constexpr int V = 16 / sizeof(B), PER = kGbTile * kGbTile / V / 256;
+  VecN<B, V> v[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = (threadIdx.x + 256 * i) * V;
     const int64_t r = r0 + e / kGbTile, c = c0 + e % kGbTile;
-    tile[e % kGbTile][e / kGbTile] = r < R && c < C ? src[r * rs + c] : B(0);
+    v[i] = gb_load(src + r * rs + c, r < R ? C - c : 0);
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = (threadIdx.x + 256 * i) * V;
+#pragma unroll
+    for (int j = 0; j < V; ++j) tile[e % kGbTile + j][e / kGbTile] = v[i].v[j];
   }
   __syncthreads();
-#pragma unroll 4
-  for (int e = threadIdx.x; e < kGbTile * kGbTile; e += 256) {
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = (threadIdx.x + 256 * i) * V;
     const int64_t c = c0 + e / kGbTile, r = r0 + e % kGbTile;
-    if (c < C && r < ld) dst[c * ld + r] = tile[e / kGbTile][e % kGbTile];
+    VecN<B, V> o;
+#pragma unroll
+    for (int j = 0; j < V; ++j) o.v[j] = tile[e / kGbTile][e % kGbTile + j];
+    if (c < C && r < ld) st<B, V>(dst + c * ld + r, o);  // ld is a multiple of 64
   }
 }
 
@@ -144,25 +184,29 @@ static GatedBackwardPlan plan_gated_backward(int64_t M, int64_t F, int64_t K, in
 template <typename T>
 static int run_dpre(const void* dhv, const void* prev, void* dpre, int64_t ld, void* dpre_t, int64_t ld_t, int64_t M, int64_t F, int act, hipStream_t st) {
   const T *dh = static_cast<const T*>(dhv), *pre = static_cast<const T*>(prev);
-  constexpr int V = 16 / sizeof(T);
-  const bool vec = F % V == 0 && ld % V == 0 && aligned16(dh) && aligned16(pre);
   // (the transpose is padded past the last row's tile when its rows are padded to more than one)
-  const int64_t tiles_f = (F + kGbTile - 1) / kGbTile, tiles_m = ((dpre_t != nullptr ? ld_t : M) + kGbTile - 1) / kGbTile;
+  const int64_t rows = dpre_t != nullptr ? ld_t : M, tiles_f = (F + kGbTile - 1) / kGbTile;
+  const bool small = tiles_f * ((rows + kGbTile - 1) / kGbTile) < kNumCU;
+  const int64_t tiles_m = small ? (rows + 15) / 16 : (rows + kGbTile - 1) / kGbTile;
   MI355_REQUIRE(tiles_f * tiles_m < (int64_t(1) << 24), "mi355_gated_linear_backward: M=%lld F=%lld is too large", (long long)M, (long long)F);
-  auto go = [&](auto a, auto row, auto col, auto v) {
-    hipLaunchKernelGGL((gated_dpre_kernel<T, decltype(a)::value, decltype(row)::value, decltype(col)::value, decltype(v)::value>),
+  auto launch = [&](auto a, auto row, auto col, auto tm) {
+    hipLaunchKernelGGL((gated_dpre_kernel<T, decltype(a)::value, decltype(row)::value, decltype(col)::value, decltype(tm)::value>),
                        dim3((unsigned)(tiles_f * tiles_m)), dim3(256), 0, st, dh, pre, static_cast<T*>(dpre), ld, static_cast<T*>(dpre_t), ld_t, M, F,
                        (int)tiles_f);
+  };
+  auto go = [&](auto a, auto row, auto col) {
+    small ? launch(a, row, col, std::integral_constant<int, 16>()) : launch(a, row, col, std::integral_constant<int, kGbTile>());
   };
   using std::false_type;
   using std::true_type;
   return dispatch_act(act, "mi355_gated_linear_backward", [&](auto a) {
-    auto parts = [&](auto v) {
-      if (dpre != nullptr && dpre_t != nullptr) go(a, true_type(), true_type(), v);
-      else if (dpre != nullptr) go(a, true_type(), false_type(), v);
-      else go(a, false_type(), true_type(), v);
-    };
-    vec ? parts(true_type()) : parts(false_type());
+    if constexpr (std::is_same<T, double>::value) {
+      go(a, true_type(), false_type());  // (no transpose: the fp64 product takes any strides)
+    } else {
+      if (dpre != nullptr && dpre_t != nullptr) go(a, true_type(), true_type());
+      else if (dpre != nullptr) go(a, true_type(), false_type());
+      else go(a, false_type(), true_type());
+    }
   });
 }
 

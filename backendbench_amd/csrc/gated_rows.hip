@@ -327,8 +327,9 @@ template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t 
     const auto kern = gated_rows_lds_kernel<T, MB, RB>;
     constexpr int bytes = 2 * RB * 16 * kRlRowBytes;
     static_assert(bytes >= kRlWaves * RB * MB * kWave * 16, "the accumulators meet in the buffers");
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != hipSuccess) return set_error(MI355_ERR_LAUNCH, "mi355_gated_linear: cannot reserve %d bytes of LDS: %s", bytes, hipGetErrorString(e));
+    static std::atomic<uint64_t> devices{0};
+    const int rc = allow_lds(reinterpret_cast<const void*>(kern), bytes, devices, "mi355_gated_linear");
+    if (rc != MI355_OK) return rc;
     hipLaunchKernelGGL(kern, dim3((unsigned)((a.F + 8 * RB - 1) / (8 * RB))), dim3(64 * kRlWaves), bytes, st, a);
     return check_launch("mi355_gated_linear");
   };

@@ -91,8 +91,9 @@ static int run_gated_x16(const GatedArgs& a, hipStream_t st) {
   const int64_t tiles = (int64_t)g.tiles_m * g.tiles_n;
   GatedStore out{a.h, a.pre, a.act, a.F % 8 == 0 && aligned16(a.h) && aligned16(a.pre)};
   const auto kern = gated_x16_kernel<T>;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kX16Lds);
-  if (e != hipSuccess) return set_error(MI355_ERR_LAUNCH, "mi355_gated_linear: cannot reserve %d bytes of LDS: %s", kX16Lds, hipGetErrorString(e));
+  static std::atomic<uint64_t> devices{0};
+  const int rc = allow_lds(reinterpret_cast<const void*>(kern), kX16Lds, devices, "mi355_gated_linear");
+  if (rc != MI355_OK) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(256), kX16Lds, st, g, out);
   return check_launch("mi355_gated_linear");
 }

@@ -1889,8 +1889,9 @@ template <typename T> static int run_gated_small2(const GatedArgs& a, hipStream_
   const int64_t warm = idle >= 16 && a.K >= 1024 ? (idle < 32 ? idle : 32) : 0;
   const GatedStore32 out{a.h, a.pre, a.act, a.F % 8 == 0 && aligned16(a.h) && aligned16(a.pre)};
   const auto kern = gated_small2_kernel<T>;
-  const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, kSmall2Lds);
-  if (e != hipSuccess) return set_error(MI355_ERR_LAUNCH, "mi355_gated_linear: cannot reserve %d bytes of LDS: %s", kSmall2Lds, hipGetErrorString(e));
+  static std::atomic<uint64_t> devices{0};
+  const int rc = allow_lds(reinterpret_cast<const void*>(kern), kSmall2Lds, devices, "mi355_gated_linear");
+  if (rc != MI355_OK) return rc;
   hipLaunchKernelGGL(kern, dim3((unsigned)(tiles + warm)), dim3(256), kSmall2Lds, st, g, out);
   return check_launch("mi355_gated_linear");
 }

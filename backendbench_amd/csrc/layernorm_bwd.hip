@@ -399,10 +399,11 @@ template <typename T> static LbTile lb_tile(int64_t N) {
   if (sizeof(T) == 4 && N <= (int64_t)kLbTile * V * 4) return LbTile{kLbTile, 4};
   return LbTile{0, 0};
 }
+// One block where four trips of it do: the finish pass is another launch (3 us), a trip about one.
 static int64_t lb_tile_blocks(int64_t M, const LbTile& p) {
   const int64_t rows = kLbTile / p.lanes;  // per block and trip
   const int64_t need = (M + rows - 1) / rows;
-  return need < kLbTileBlocks ? need : kLbTileBlocks;
+  return need <= 4 ? 1 : need < kLbTileBlocks ? need : kLbTileBlocks;
 }
 
 template <typename T, typename Wt, int V, int GL, int NV, bool TAIL>
@@ -412,8 +413,9 @@ static int launch_lb_tile(int64_t blocks, const T* dy, const T* x, const float* 
   constexpr int bytes = WG > 1 ? 2 * WG * NV * GL * V * (int)sizeof(float) : 0;
   const auto kern = lb_tile_kernel<T, Wt, V, GL, NV, TAIL>;
   if (bytes > 48 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != hipSuccess) return set_error(MI355_ERR_LAUNCH, "mi355_layer_norm_backward: cannot reserve %d bytes of LDS: %s", bytes, hipGetErrorString(e));
+    static std::atomic<uint64_t> devices{0};
+    const int rc = allow_lds(reinterpret_cast<const void*>(kern), bytes, devices, "mi355_layer_norm_backward");
+    if (rc != MI355_OK) return rc;
   }
   hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3(kLbTile), bytes, st, dy, x, mean, rstd, w, dx, partial, dw, db, M, (int)N);
   return check_launch("mi355_layer_norm_backward");
@@ -476,7 +478,7 @@ using namespace mi355;
 extern "C" int64_t mi355_layer_norm_backward_workspace_bytes(int64_t M, int64_t N, int dtype) {
   if (M <= 0 || N <= 0 || dtype_size(dtype) == 0) return 0;
   const LbTile p = dtype == MI355_F32 ? lb_tile<float>(N) : dtype == MI355_F64 ? lb_tile<double>(N) : lb_tile<bf16_t>(N);
-  if (p.lanes != 0) return lb_tile_blocks(M, p) * 2 * lb_ld(N) * 4;
+  if (p.lanes != 0) return lb_tile_blocks(M, p) > 1 ? lb_tile_blocks(M, p) * 2 * lb_ld(N) * 4 : 0;
   return (2 * M + lb_plan(M, N).groups * 2 * lb_ld(N)) * (dtype == MI355_F64 ? 8 : 4);
 }
 
@@ -490,9 +492,9 @@ extern "C" int mi355_layer_norm_backward(const void* dy, const void* x, int dtyp
   MI355_REQUIRE(dy != nullptr && x != nullptr && mean != nullptr && rstd != nullptr, "mi355_layer_norm_backward: NULL data pointer");
   MI355_REQUIRE(M < (int64_t(1) << 40) && N < (int64_t(1) << 28), "mi355_layer_norm_backward: extents too large (M=%lld N=%lld)",
                 (long long)M, (long long)N);
-  MI355_REQUIRE(workspace != nullptr && workspace_bytes >= mi355_layer_norm_backward_workspace_bytes(M, N, dtype) && aligned16(workspace),
-                "mi355_layer_norm_backward: needs a 16-byte aligned workspace of %lld bytes",
-                (long long)mi355_layer_norm_backward_workspace_bytes(M, N, dtype));
+  const int64_t need = mi355_layer_norm_backward_workspace_bytes(M, N, dtype);
+  MI355_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need && aligned16(workspace)),
+                "mi355_layer_norm_backward: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define MI355_LB(DT, WDT, T_, W_, S_) \
   if (dtype == DT && w_dtype == WDT) return run_lb<T_, W_, S_>(dy, x, mean, rstd, weight, dx, dweight, dbias, M, N, workspace, st);

@@ -70,23 +70,34 @@ def device_managed(fn):
     return wrapper
 
 
-def on_device_of_arguments(fn):
-    """Run `fn` with the GPU of its tensor arguments current, so that its launches go to that GPU's current stream;
-    tensors on more than one GPU are refused.  Goes under device_managed, which brings every tensor to a GPU."""
+def on_gpu(fn):
+    """device_managed for the operators that also follow their tensors: `fn` runs with the GPU of its arguments current, so
+    that its launches go to that GPU's current stream; tensors on more than one GPU are refused.  Positional arguments only.
+    The common case, everything on the current GPU, is one look at each tensor."""
 
     @functools.wraps(fn)
-    def wrapper(*args, **kwargs):
+    def one_device(*args):
         device = None
-        for a in (*args, *kwargs.values()):
+        for a in args:
             if isinstance(a, torch.Tensor):
                 if device is None:
                     device = a.device
                 elif a.device != device:
                     raise RuntimeError(f"Expected all tensors to be on the same device, but found at least two devices, {device} and {a.device}!")
-        if device is None or device.index == _current_device():
-            return fn(*args, **kwargs)
         with torch.cuda.device(device):
-            return fn(*args, **kwargs)
+            return fn(*args)
+
+    anywhere = device_managed(one_device)
+
+    @functools.wraps(fn)
+    def wrapper(*args):
+        if torch.cuda.is_initialized():
+            current = _current_device()
+            for a in args:
+                if isinstance(a, torch.Tensor) and a.get_device() != current:
+                    return anywhere(*args)
+            return fn(*args)
+        return anywhere(*args)
 
     return wrapper
 

@@ -8,8 +8,7 @@ a call of the operator that computes it.  Arguments are checked before anything 
 import torch
 
 from .. import _lib
-from ._common import (cast, copy_into, dense, device_managed, launch, new_dense, new_result, on_device_of_arguments, prod,
-                      try_launch)
+from ._common import cast, copy_into, dense, launch, new_dense, new_result, on_gpu, prod, try_launch
 from .elementwise import _store_result as store_result
 from .elementwise import tuple_out_variant
 from .matmul import _gemm, _gemm_f32out
@@ -23,75 +22,85 @@ def _need_float(t, what):
         raise NotImplementedError(f"mi355 backend: {what} on {t.dtype} is not supported")
 
 
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
 # ---- layer norm, backward ------------------------------------------------------------------------------------------
 def native_layer_norm_backward(grad_out, input, normalized_shape, mean, rstd, weight, bias, output_mask):
     """aten.native_layer_norm_backward.default -> (grad_input, grad_weight, grad_bias), None where output_mask is False.
 
     mean and rstd are what native_layer_norm returned; grad_weight and grad_bias have the dtype of weight and bias."""
-    k = len(normalized_shape)
-    if k == 0 or list(input.shape[input.dim() - k :]) != list(normalized_shape):
+    k, shape = len(normalized_shape), input.shape
+    if k == 0 or k > len(shape) or shape[len(shape) - k :] != tuple(normalized_shape):
         raise RuntimeError(
             f"Given normalized_shape={list(normalized_shape)}, expected input with shape "
-            f"[*, {', '.join(str(s) for s in normalized_shape)}], but got input of size{list(input.shape)}")
+            f"[*, {', '.join(str(s) for s in normalized_shape)}], but got input of size{list(shape)}")
     _need_float(input, "layer norm")
-    if grad_out.shape != input.shape:
-        raise RuntimeError(f"Expected grad_out of the input's shape {list(input.shape)}, but got {list(grad_out.shape)}")
+    if grad_out.shape != shape:
+        raise RuntimeError(f"Expected grad_out of the input's shape {list(shape)}, but got {list(grad_out.shape)}")
     if grad_out.dtype != input.dtype:
         raise RuntimeError(f"Expected grad_out of the input's dtype {input.dtype}, but got {grad_out.dtype}")
-    M = prod(input.shape[: input.dim() - k])
+    M = prod(shape[: len(shape) - k])
     for name, s in (("mean", mean), ("rstd", rstd)):
         if s.numel() != M:
             raise RuntimeError(f"Expected {name} to hold {M} values, one per row, but got {s.numel()}")
-        _need_float(s, f"layer norm statistics ({name})")
-    for i, (name, p) in enumerate((("weight", weight), ("bias", bias))):
+        _need_float(s, name)
+    for name, p, wanted in (("weight", weight, output_mask[1]), ("bias", bias, output_mask[2])):
         if p is None:
-            if output_mask[i + 1]:
+            if wanted:
                 raise RuntimeError(f"the gradient of {name} was asked for, but {name} is None")
-        elif list(p.shape) != list(normalized_shape):
+        elif p.shape != tuple(normalized_shape):
             raise RuntimeError(f"Expected {name} to be of same shape as normalized_shape, but got {name} of shape "
                                f"{list(p.shape)} and normalized_shape = {list(normalized_shape)}")
         else:
-            _need_float(p, f"layer norm {name}")
+            _need_float(p, name)
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise RuntimeError("weight and bias must have the same dtype")
-    return _layer_norm_backward(grad_out, input, list(normalized_shape), mean, rstd, weight, bias, [bool(v) for v in output_mask])
+    return _layer_norm_backward(grad_out, input, mean, rstd, weight, bias, M, tuple(normalized_shape), output_mask)
 
 
-@device_managed
-@on_device_of_arguments
-def _layer_norm_backward(grad_out, input, normalized_shape, mean, rstd, weight, bias, mask):
-    k = len(normalized_shape)
-    M, N = prod(input.shape[: input.dim() - k]), prod(normalized_shape)
-    w_given = weight.dtype if weight is not None else bias.dtype if bias is not None else input.dtype
-    dx = new_result(input.shape, input.dtype, input.device) if mask[0] else None
-    grads = [new_result(normalized_shape, w_given, input.device) if m else None for m in mask[1:]]
-    if M == 0 or N == 0 or not any(mask):
-        for g in grads:
+_ln_workspace = None
+
+
+@on_gpu
+def _layer_norm_backward(grad_out, input, mean, rstd, weight, bias, M, normalized_shape, mask):
+    global _ln_workspace
+    N = prod(normalized_shape)
+    dtype, device = input.dtype, input.device
+    w_given = weight.dtype if weight is not None else bias.dtype if bias is not None else dtype
+    dx = new_result(input.shape, dtype, device) if mask[0] else None
+    dw = new_result(normalized_shape, w_given, device) if mask[1] else None
+    db = new_result(normalized_shape, w_given, device) if mask[2] else None
+    if M == 0 or N == 0 or not (mask[0] or mask[1] or mask[2]):
+        for g in (dw, db):
             if g is not None:
                 g.zero_()
-        return dx, grads[0], grads[1]
+        return dx, dw, db
     # the kernels take parameters of the rows' dtype, or fp32 beside bf16 / f16 rows
-    w_dtype = w_given if w_given == input.dtype or (w_given == torch.float32 and input.dtype in _HALF) else input.dtype
-    if w_dtype != w_given and input.dtype in _HALF:
-        w_dtype = torch.float32  # (fp64 or the other half type: through fp32, not through the narrower type)
-    stat_dtype = torch.float64 if input.dtype == torch.float64 else torch.float32
+    w_dtype = w_given
+    if w_given != dtype:
+        w_dtype = torch.float32 if dtype in _HALF else dtype  # (never through a type narrower than both)
+    stat_dtype = torch.float64 if dtype == torch.float64 else torch.float32
     x, dy = dense(input), dense(grad_out)
     mu, rs = dense(cast(mean, stat_dtype)), dense(cast(rstd, stat_dtype))
     w = dense(cast(weight, w_dtype)) if weight is not None else None
-    outs = [g if g is None or g.dtype == w_dtype else new_dense(g.shape, w_dtype, g.device) for g in grads]
-    code = _lib.dtype_code(input.dtype)
-    ws_bytes = _lib.load().mi355_layer_norm_backward_workspace_bytes(M, N, code)
-    ws = new_dense((ws_bytes,), torch.uint8, input.device)
-
-    def ptr(t):
-        return t.data_ptr() if t is not None else None
-
-    launch("mi355_layer_norm_backward", dy.data_ptr(), x.data_ptr(), code, mu.data_ptr(), rs.data_ptr(), ptr(w),
-           _lib.dtype_code(w_dtype), ptr(dx), ptr(outs[0]), ptr(outs[1]), M, N, ws.data_ptr(), ws_bytes)
-    for g, o in zip(grads, outs):
-        if g is not o:
-            copy_into(g, o)
-    return dx, grads[0], grads[1]
+    own_dw, own_db = dw, db  # what the kernel writes
+    if w_given != w_dtype:
+        own_dw = new_dense(normalized_shape, w_dtype, device) if mask[1] else None
+        own_db = new_dense(normalized_shape, w_dtype, device) if mask[2] else None
+    code = _lib.DTYPE[dtype]
+    if _ln_workspace is None:
+        _ln_workspace = _lib.load().mi355_layer_norm_backward_workspace_bytes
+    ws_bytes = _ln_workspace(M, N, code)
+    ws = new_dense((ws_bytes,), torch.uint8, device) if ws_bytes else None
+    launch("mi355_layer_norm_backward", dy.data_ptr(), x.data_ptr(), code, mu.data_ptr(), rs.data_ptr(), _ptr(w),
+           _lib.DTYPE[w_dtype], _ptr(dx), _ptr(own_dw), _ptr(own_db), M, N, _ptr(ws), ws_bytes)
+    if dw is not own_dw:
+        copy_into(dw, own_dw)
+    if db is not own_db:
+        copy_into(db, own_db)
+    return dx, dw, db
 
 
 _out_all = tuple_out_variant(native_layer_norm_backward, 3)
@@ -130,41 +139,49 @@ def gated_linear(input, weight, activation="silu", save_pre=False):
     fp64) and not rounded before the activation.  save_pre: also return the pre-activations [..., 2F] in the input's
     dtype, which gated_linear_backward takes; the one rounding between the two passes."""
     _check_gated(input, weight, activation)
-    return _gated_linear(input, weight, activation, bool(save_pre))
+    return _gated_linear(input, weight, _ACTIVATIONS[activation], save_pre)
 
 
 _PAD_ROWS = 64  # more rows than this are worth a zero-padded copy of a weight whose rows the kernels cannot take
 
 
+def _rows_of(t):
+    """`t` [R, K] itself when its rows are unit-stride and do not overlap, else a dense copy."""
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else dense(t)
+
+
 def _gated_fused(x, weight, h, pre, act):
     """The one-kernel form on x [M, K]; False when there is none for these operands (nothing was launched)."""
     M, K = x.shape
-    if weight.stride(1) != 1 and K > 1:
-        weight = dense(weight)
-    if M > _PAD_ROWS and (K % 128 or K < 256 or weight.stride(0) % 8 or weight.data_ptr() % 16 or x.data_ptr() % 16):
-        # copied once into rows of a multiple of 128 (exact: the pad adds 0 * 0 terms)
-        Kp = max((K + 127) // 128 * 128, 256)
-        both = torch.zeros((M + weight.shape[0], Kp), dtype=x.dtype, device=x.device)
-        copy_into(both[:M, :K], x)
-        copy_into(both[M:, :K], weight)
-        x, weight = both[:M], both[M:]
-    return try_launch("mi355_gated_linear", x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), h.data_ptr(),
-                      pre.data_ptr() if pre is not None else None, M, weight.shape[0] // 2, x.shape[1], act, _lib.dtype_code(x.dtype))
+    F = weight.shape[0] // 2
+    code = _lib.DTYPE[x.dtype]
+    weight = _rows_of(weight)
+    if try_launch("mi355_gated_linear", x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), h.data_ptr(), _ptr(pre), M, F, K,
+                  act, code):
+        return True
+    if M <= _PAD_ROWS:
+        return False
+    # copied once into aligned rows of a multiple of 128 (exact: the pad adds 0 * 0 terms)
+    Kp = max((K + 127) // 128 * 128, 256)
+    both = new_dense((M + 2 * F, Kp), x.dtype, x.device)
+    copy_into(both[:M, :K], x)
+    copy_into(both[M:, :K], weight)
+    if Kp > K:
+        both[:, K:].zero_()
+    return try_launch("mi355_gated_linear", both.data_ptr(), Kp, both[M:].data_ptr(), Kp, h.data_ptr(), _ptr(pre), M, F, Kp, act, code)
 
 
-@device_managed
-@on_device_of_arguments
-def _gated_linear(input, weight, activation, save_pre):
-    lead, K = list(input.shape[:-1]), input.shape[-1]
+@on_gpu
+def _gated_linear(input, weight, act, save_pre):
+    lead, K = input.shape[:-1], input.shape[-1]
     M, F = prod(lead), weight.shape[0] // 2
     dtype, device = input.dtype, input.device
     if M == 0 or F == 0 or K == 0:  # (no terms: pre = 0 and act(0) = 0)
-        h = torch.zeros(lead + [F], dtype=dtype, device=device)
-        return (h, torch.zeros(lead + [2 * F], dtype=dtype, device=device)) if save_pre else h
-    h = new_dense(lead + [F], dtype, device)
-    pre = new_dense(lead + [2 * F], dtype, device) if save_pre else None
-    act = _ACTIVATIONS[activation]
-    x = dense(input).view(M, K)
+        h = torch.zeros((*lead, F), dtype=dtype, device=device)
+        return (h, torch.zeros((*lead, 2 * F), dtype=dtype, device=device)) if save_pre else h
+    h = new_dense((*lead, F), dtype, device)
+    pre = new_dense((*lead, 2 * F), dtype, device) if save_pre and dtype in _HALF else None
+    x = _rows_of(input) if input.dim() == 2 else dense(input).view(M, K)
     if dtype in _HALF:
         if _gated_fused(x, weight, h, pre, act):
             return (h, pre) if save_pre else h
@@ -172,9 +189,9 @@ def _gated_linear(input, weight, activation, save_pre):
     else:
         wide, saved = _gemm(x, weight.t(), None, 1.0, 0.0), None
         if save_pre:
-            pre = wide.view(lead + [2 * F])
+            pre = wide.view(*lead, 2 * F)
     launch("mi355_gated_act", wide.data_ptr(), _lib.dtype_code(wide.dtype), h.data_ptr(),
-           saved.data_ptr() if saved is not None else None, _lib.dtype_code(dtype), M, F, act)
+           _ptr(saved), _lib.dtype_code(dtype), M, F, act)
     return (h, pre) if save_pre else h
 
 
@@ -193,27 +210,26 @@ def gated_linear_backward(grad_out, input, weight, pre, activation="silu", outpu
             raise RuntimeError(f"Expected {name} of the input's dtype {input.dtype}, but got {t.dtype}")
     if len(output_mask) != 2:
         raise RuntimeError(f"output_mask must have 2 entries, got {len(output_mask)}")
-    return _gated_linear_backward(grad_out, input, weight, pre, activation, [bool(v) for v in output_mask])
+    return _gated_linear_backward(grad_out, input, weight, pre, _ACTIVATIONS[activation], output_mask)
 
 
-@device_managed
-@on_device_of_arguments
-def _gated_linear_backward(grad_out, input, weight, pre, activation, mask):
+@on_gpu
+def _gated_linear_backward(grad_out, input, weight, pre, act, mask):
     K, F = weight.shape[1], weight.shape[0] // 2
     M = prod(input.shape[:-1])
     dtype, device = input.dtype, input.device
-    if M == 0 or F == 0 or K == 0 or not any(mask):
+    if M == 0 or F == 0 or K == 0 or not (mask[0] or mask[1]):
         return (torch.zeros_like(input) if mask[0] else None), (torch.zeros_like(weight) if mask[1] else None)
-    dh, p, x = dense(grad_out), dense(pre), dense(input)
-    w = weight if weight.stride(1) == 1 and weight.stride(0) >= K else dense(weight)
+    dh, p = dense(grad_out), dense(pre)
+    x = _rows_of(input) if input.dim() == 2 else dense(input).view(M, K)
+    w = _rows_of(weight)
     dx = new_dense(input.shape, dtype, device) if mask[0] else None
     dw = new_dense(weight.shape, dtype, device) if mask[1] else None
     code = _lib.dtype_code(dtype)
     ws_bytes = _lib.load().mi355_gated_linear_backward_workspace_bytes(M, F, K, code)
     ws = new_dense((ws_bytes,), torch.uint8, device)
-    launch("mi355_gated_linear_backward", dh.data_ptr(), x.data_ptr(), K, w.data_ptr(), w.stride(0), p.data_ptr(),
-           dx.data_ptr() if mask[0] else None, dw.data_ptr() if mask[1] else None, M, F, K, _ACTIVATIONS[activation], code,
-           ws.data_ptr(), ws_bytes)
+    launch("mi355_gated_linear_backward", dh.data_ptr(), x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), p.data_ptr(),
+           _ptr(dx), _ptr(dw), M, F, K, act, code, ws.data_ptr(), ws_bytes)
     return dx, dw
 
 
@@ -259,8 +275,7 @@ def _int64(v):
     return (int(v) + 2 ** 63) % 2 ** 64 - 2 ** 63
 
 
-@device_managed
-@on_device_of_arguments
+@on_gpu
 def _dropout_add(input, residual, p, rng):
     out = new_dense(input.shape, input.dtype, input.device)
     if input.numel() == 0:
@@ -272,6 +287,5 @@ def _dropout_add(input, residual, p, rng):
         words = dense(rng)
     else:
         seed, offset = (_int64(v) for v in rng)
-    launch("mi355_dropout_add", x.data_ptr(), res.data_ptr() if res is not None else None, _lib.dtype_code(x.dtype), p,
-           words.data_ptr() if words is not None else None, seed, offset, out.data_ptr(), x.numel())
+    launch("mi355_dropout_add", x.data_ptr(), _ptr(res), _lib.DTYPE[x.dtype], p, _ptr(words), seed, offset, out.data_ptr(), x.numel())
     return out

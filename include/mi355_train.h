@@ -21,7 +21,7 @@ extern "C" {
  * dbias: `w_dtype` (dtype, or f32 for f16 / bf16 rows); mean, rstd: M values each, f32 (f64 for f64 rows).  Sums are
  * held in fp32 (fp64 for f64 rows) and added in a fixed order: the same call gives the same bits.
  * The workspace (contents undefined before and after) must hold mi355_layer_norm_backward_workspace_bytes() bytes,
- * 16-byte aligned; a call with less is refused.
+ * 16-byte aligned (0 for a handful of rows: NULL is accepted); a call with less is refused.
  * Slot: native_layer_norm_backward__default. */
 int64_t mi355_layer_norm_backward_workspace_bytes(int64_t M, int64_t N, int dtype);
 int mi355_layer_norm_backward(const void* dy, const void* x, int dtype, const void* mean, const void* rstd,
@@ -39,8 +39,8 @@ typedef enum mi355_activation {
 /* h = act(x Wg^T) * (x Wu^T) in one kernel: x [M][K] with rows x_rs apart, weight [2F][K] = [Wg; Wu] with rows w_rs
  * apart, both unit-stride along K; h [M][F] dense; pre (may be NULL) receives the pre-activations [M][2F], dense.  All of
  * `dtype`.  Products accumulate in fp32; the activation takes the unrounded sums.  For f16 / bf16: up to 64 rows
- * with any K, strides and alignment; more rows with 16-byte aligned rows of K % 128 == 0, K >= 256.  Otherwise
- * MI355_ERR_UNSUPPORTED with nothing launched (a product and mi355_gated_act do it). */
+ * with any K, strides and alignment; more with 16-byte aligned rows of K % 128 == 0, K >= 256 (K % 64 == 0
+ * where (M / 128) (F / 64) tiles are at most 512).  Otherwise MI355_ERR_UNSUPPORTED with nothing launched (a product and mi355_gated_act do it). */
 int mi355_gated_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, void* h, void* pre, int64_t M, int64_t F,
                        int64_t K, int act, int dtype, void* stream);
 

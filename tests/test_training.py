@@ -128,11 +128,12 @@ def test_c_entry_points_check_their_arguments():
         assert rc < 0 and text in lib.mi355_last_error(), (rc, lib.mi355_last_error())
 
     ln = lib.mi355_layer_norm_backward
-    need = lib.mi355_layer_norm_backward_workspace_bytes(4, 8, _lib.F32)
+    assert lib.mi355_layer_norm_backward_workspace_bytes(4, 8, _lib.F32) == 0    # one block holds it all
+    need = lib.mi355_layer_norm_backward_workspace_bytes(4000, 8, _lib.F32)
     assert need > 0
-    refused(ln(p, p, _lib.F32, p, p, p, _lib.F32, p, p, p, 4, 8, p, need - 1, None), b"workspace")
-    refused(ln(p, p, _lib.F32, p, p, p, _lib.F32, p, p, p, 4, 8, None, need, None), b"workspace")
-    refused(ln(p, p, _lib.F32, p, p, p, _lib.F32, p, p, p, 4, 8, p + 4, need, None), b"workspace")
+    refused(ln(p, p, _lib.F32, p, p, p, _lib.F32, p, p, p, 4000, 8, p, need - 1, None), b"workspace")
+    refused(ln(p, p, _lib.F32, p, p, p, _lib.F32, p, p, p, 4000, 8, None, need, None), b"workspace")
+    refused(ln(p, p, _lib.F32, p, p, p, _lib.F32, p, p, p, 4000, 8, p + 4, need, None), b"workspace")
     refused(ln(None, p, _lib.F32, p, p, p, _lib.F32, p, p, p, 4, 8, p, need, None), b"NULL")
     refused(ln(p, p, _lib.F32, p, p, p, _lib.F32, p, p, p, -1, 8, p, need, None), b"negative")
     refused(ln(p, p, _lib.F32, p, p, p, _lib.F32, p, p, p, 0, 8, p, need, None), b"no rows")

@@ -318,6 +318,12 @@ def test_gated_linear_shapes_strides_and_masks():
     sliced = randn(g, 9, 300, dtype=torch.float16)[:, 4:260]                       # rows 300 apart, 8 bytes off a boundary
     ws = randn(g, 96, 264, dtype=torch.float16, scale=0.1)[:, :256]
     gated_forward_check(ops.gated_linear(sliced, ws, "gelu"), None, sliced.contiguous(), ws.contiguous(), "gelu", "sliced")
+    # overlapping rows: a weight whose rows are all the same storage, tokens that share elements
+    same = randn(g, 1, 256, dtype=torch.float16, scale=0.1).expand(64, 256)
+    shared = randn(g, 1000, dtype=torch.float16).as_strided((90, 256), (8, 1))
+    gated_forward_check(ops.gated_linear(shared, same, "silu"), None, shared.contiguous(), same.contiguous(), "silu", "overlapping")
+    dx, dw = ops.gated_linear_backward(shared[:, :32], shared, same, shared[:, :64], "silu")
+    gated_backward_check((dx, dw), shared[:, :32].contiguous(), shared.contiguous(), same.contiguous(), shared[:, :64].contiguous(), "silu", "overlapping")
 
 
 def test_gated_linear_empties():
