@@ -10,6 +10,12 @@ namespace mi355 {
 
 typedef uint32_t gr_any __attribute__((ext_vector_type(4), aligned(2)));  // 8 elements at any element's address
 
+// Behind the last matrix instruction on `v`, in front of its first other reader: 16 wait states, more than the 16x16x32
+// instruction needs.  Not left to the compiler: in the LDS kernel's branch for K under a chunk it put none between the last
+// v_mfma and the ds_write of its result, and the write took the registers' old contents (the generated code shows it, and
+// [3, 1000] x 2 * 24 f16 came out wrong).
+__device__ __forceinline__ void settle(f32x4& v) { asm volatile("s_nop 15" : "+v"(v)); }
+
 template <typename T> struct GrMfma;
 template <> struct GrMfma<bf16_t> {
   static __device__ __forceinline__ f32x4 run(u32x4 a, u32x4 b, f32x4 c) {
@@ -46,124 +52,139 @@ template <typename T> __device__ __forceinline__ void store_rows(const GatedArgs
     }
 }
 
-// Aligned rows: the weight goes through LDS.  An MFMA fragment takes 64 bytes of each of 16 rows per load instruction; the
-// memory system delivers such requests at 4.6 - 5.0 TB/s whatever their order, and pieces of 1 KB of one row, 2 KB of a row
-// per workgroup at a time, at 6.3 - 6.5 (a [22016, 4096] weight read by nothing but loads).  So the rows are requested in
-// 1 KB pieces straight into LDS (global_load_lds), two buffers of kRlChunk elements of each row, and the fragments are read
-// from there: 16-byte unit c of row r sits at c ^ (r % 16), so that the 16 rows of a fragment read fall into 16 distinct
-// columns of the 256-byte bank window.  Eight waves share a buffer, each takes its eighth of the chunk's k for all RB x 8
-// features (8 gate rows and the 8 up rows of the same features make one 16-row operand) and MB x 16 tokens; x comes
-// straight from L2 in fragments, one chunk ahead.
-constexpr int kRlChunk = 1024, kRlWaves = 8;
-constexpr int kRlRowBytes = kRlChunk * 2;
+// Aligned rows: weight and x go through LDS.  An MFMA fragment takes 64 bytes of each of 16 rows per load instruction; the
+// memory system delivers such requests at 4.6 - 5.0 TB/s whatever their order, and 1 KB pieces of one row at 6.4 (a [22016,
+// 4096] weight read by nothing but loads: 36 - 39 us against 28).  So both operands are requested in whole pieces straight
+// into LDS (global_load_lds, 64 units of 16 bytes), a ring of NB buffers of KC elements of each row deep, and the fragments
+// are read from there: unit c of row r sits at c ^ (r % 16), so that the 16 rows of a fragment read fall into 16 distinct
+// columns of the 256-byte bank window.  Everything that is in flight is a request of one kind, counted by hand: a load into
+// registers between them would have to be waited for together with all older requests.
+// A block is RB x 8 features: their gate rows and the up rows of the same features, 8 + 8, make one 16-row operand; eight
+// waves share it, each takes an eighth of a buffer's k.  RX rows of x are staged (fewer tokens than RX: the last one again).
+constexpr int kRlWaves = 8;
 
-template <typename T, int MB, int RB>
-__global__ __launch_bounds__(64 * kRlWaves, RB == 1 ? 4 : 2) void gated_rows_lds_kernel(GatedArgs g) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // two buffers; at the end the waves' accumulators
-  constexpr int BUF = RB * 16 * kRlRowBytes;
-  constexpr int FILLS = RB * 4;  // 1 KB requests of a wave per buffer: RB x 32 in all
-  constexpr int P = kRlChunk / kRlWaves / 32;  // 32-k pieces of a wave per chunk
+// A request with the streaming hint (a weight is read once per call) or without.
+template <bool STREAM> __device__ __forceinline__ void rl_fill(uint32_t lds_byte_offset, uint32_t lane_byte_offset, const void* base) {
+  if constexpr (STREAM)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds_byte_offset), "v"(lane_byte_offset), "s"(base) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_byte_offset), "v"(lane_byte_offset), "s"(base) : "memory");
+}
+template <int N> __device__ __forceinline__ void rl_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+template <typename T, int RX, int RB, int KC, int NB> struct RowsShape {
+  static constexpr int MB = (RX + 15) / 16;            // token blocks
+  static constexpr int ROWS = 16 * RB;                 // weight rows of a block
+  static constexpr int UNITS = KC / 8;                 // 16-byte units of a row
+  static constexpr int RPI = 64 / UNITS;               // rows per request
+  static constexpr int WFILLS = ROWS / RPI / kRlWaves;                               // requests of a wave per buffer: weight,
+  static constexpr int XFILLS = RX / RPI >= kRlWaves ? RX / RPI / kRlWaves : 1;      // x (fewer than waves: some twice)
+  static constexpr int FILLS = WFILLS + XFILLS;
+  static constexpr int P = KC / kRlWaves / 32;         // 32-k pieces of a wave per buffer
+  static constexpr int BUF = (ROWS + RX) * KC * 2;
+  static constexpr int MEET = kRlWaves * RB * MB * kWave * 16;
+  static constexpr int LDS = NB * BUF > MEET ? NB * BUF : MEET;
+};
+
+template <typename T, int RX, int RB, int KC, int NB, int WAVES_PER_SIMD>
+__global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_kernel(GatedArgs g) {
+  using S = RowsShape<T, RX, RB, KC, NB>;
+  constexpr int MB = S::MB, P = S::P, UNITS = S::UNITS, RPI = S::RPI;
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // the ring; at the end the waves' accumulators
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lr = lane & 15, lg = lane >> 4;
-  const int64_t f0 = (int64_t)blockIdx.x * (8 * RB);
   const uint32_t lds_base = (uint32_t)(uintptr_t)lds;
-  // Row r (0 .. 16 RB - 1) of the workgroup: feature f0 + 8 (r / 16) + r % 8, its gate row when r % 16 < 8, else its up row;
-  // features past the last are computed on the last one's rows and not stored.
+  const int64_t f0 = (int64_t)blockIdx.x * (8 * RB);
+  // Row r of the block: feature f0 + 8 (r / 16) + r % 8, its gate row when r % 16 < 8, else its up row; features past the last
+  // are computed on the last one's rows and not stored.
   auto row_of = [&](int r) {
     int64_t f = f0 + 8 * (r >> 4) + (r & 7);
     f = f < g.F ? f : g.F - 1;
-    return static_cast<const T*>(g.w) + ((r & 8) ? g.F + f : f) * g.w_rs;
+    return ((r & 8) ? g.F + f : f) * g.w_rs;
   };
-  const T* xrow[MB];
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    const int64_t m = mb * 16 + lr;
-    xrow[mb] = static_cast<const T*>(g.x) + (m < g.M ? m : g.M - 1) * g.x_rs;
-  }
-  const int chunks = (int)(g.K / kRlChunk);
+  const T* W = static_cast<const T*>(g.w);
+  const T* X = static_cast<const T*>(g.x);
+  const int chunks = (int)(g.K / KC);
   // Rows are usually a power of two apart, so the memory channel of a piece is a matter of its k: workgroups that share an
   // L2 (every eighth) start at different chunks.
   const int turn = chunks > 0 ? (int)(blockIdx.x / kNumXCD % chunks) : 0;
-  auto k_of = [&](int i) { return (int64_t)(i + turn < chunks ? i + turn : i + turn - chunks) * kRlChunk; };
-  auto fill = [&](int i, int buf) {
-    const int64_t k = k_of(i);
+  // A request covers RPI rows; lane l fetches unit (l % UNITS) ^ (r % 16) of row r = first + l / UNITS, which lands at l.
+  auto fill = [&](int c) {
+    const int64_t k = (int64_t)(c + turn < chunks ? c + turn : c + turn - chunks) * KC;
+    const uint32_t buf = lds_base + (uint32_t)(c % NB) * S::BUF;
 #pragma unroll
-    for (int q = 0; q < FILLS; ++q) {
-      const int piece = wave * FILLS + q, r = piece >> 1, half = piece & 1;
-      lds_dma16s(lds_base + (uint32_t)(buf * BUF + piece * 1024), (uint32_t)((lane ^ (r & 15)) * 16), row_of(r) + k + half * 512);
+    for (int q = 0; q < S::WFILLS; ++q) {
+      const int first = (wave * S::WFILLS + q) * RPI;
+      const int64_t row0 = row_of(first);
+      uint32_t off = (uint32_t)(((lane % UNITS) ^ ((first + lane / UNITS) & 15)) * 16);
+      if constexpr (RPI > 1) off += lane / UNITS ? (uint32_t)((row_of(first + 1) - row0) * 2) : 0u;  // (rows 2 i, 2 i + 1: neighbours)
+      rl_fill<true>(buf + first * (KC * 2), off, W + row0 + k);
     }
-  };
-  auto fetch_x = [&](int i, u32x4 (&x)[MB][P]) {
-    const int64_t k = k_of(i) + wave * (32 * P) + 8 * lg;
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-      for (int p = 0; p < P; ++p) x[mb][p] = *reinterpret_cast<const u32x4*>(xrow[mb] + k + 32 * p);
+    for (int q = 0; q < S::XFILLS; ++q) {
+      const int first = (wave * S::XFILLS + q) * RPI % RX;
+      const int64_t m0 = first < g.M ? first : g.M - 1, m1 = first + 1 < g.M ? first + 1 : g.M - 1;
+      uint32_t off = (uint32_t)(((lane % UNITS) ^ ((first + lane / UNITS) & 15)) * 16);
+      if constexpr (RPI > 1) off += lane / UNITS ? (uint32_t)((m1 - m0) * g.x_rs * 2) : 0u;
+      rl_fill<false>(buf + (S::ROWS + first) * (KC * 2), off, X + m0 * g.x_rs + k);
+    }
   };
   f32x4 acc[RB][MB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) acc[rb][mb] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](int buf, const u32x4 (&x)[MB][P]) {
+  auto multiply = [&](int c) {
+    const unsigned char* buf = lds + (c % NB) * S::BUF;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      const int c = wave * (4 * P) + 4 * p + lg;  // 16-byte unit of the row
+      const int u = wave * (4 * P) + 4 * p + lg;  // this lane's unit of a row
+      u32x4 x[MB];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        const int r = (mb * 16 + lr) % RX;  // (tokens past RX repeat: never stored)
+        x[mb] = *reinterpret_cast<const u32x4*>(buf + (S::ROWS + r) * (KC * 2) + ((u ^ (r & 15)) << 4));
+      }
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(lds + buf * BUF + (rb * 16 + lr) * kRlRowBytes + (c >> 6) * 1024 + (((c & 63) ^ lr) << 4));
+        const u32x4 w = *reinterpret_cast<const u32x4*>(buf + (rb * 16 + lr) * (KC * 2) + ((u ^ lr) << 4));
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) acc[rb][mb] = GrMfma<T>::run(w, x[mb][p], acc[rb][mb]);
+        for (int mb = 0; mb < MB; ++mb) acc[rb][mb] = GrMfma<T>::run(w, x[mb], acc[rb][mb]);
       }
     }
   };
-  if (chunks > 0) {
-    u32x4 xa[MB][P], xb[MB][P];
-    fetch_x(0, xa);
-    fill(0, 0);
-    // One chunk: the next one's x and weight pieces are requested, then this one's pieces waited for (all but the last FILLS
-    // requests are back: the wait covers x too) and met by every wave.  The barrier behind the multiplication frees the
-    // buffer.
-    auto chunk = [&](int i, const u32x4 (&x)[MB][P], u32x4 (&xn)[MB][P]) {
-      if (i + 1 < chunks) {
-        fetch_x(i + 1, xn);
-        asm volatile("" ::: "memory");
-        fill(i + 1, (i + 1) & 1);
-        if constexpr (FILLS == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-      } else {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      }
-      __syncthreads();
-      multiply(i & 1, x);
-      __syncthreads();
-    };
-    for (int i = 0; i < chunks; i += 2) {
-      chunk(i, xa, xb);
-      if (i + 1 < chunks) chunk(i + 1, xb, xa);
-    }
-  }
-  // What is left of K, under a chunk: 32-k pieces, four per wave at most, all requested before the first is used; rows end
-  // on a 16-byte unit, units behind the end are zeros in both operands (0 * inf).
-  const int64_t k0 = (int64_t)chunks * kRlChunk;
-  if (k0 < g.K) {
-    const T* wrow[RB];
+  // NB - 1 buffers ahead.  Chunk c: its requests are back when only those of the NB - 2 chunks behind it are out; the barrier
+  // that follows says so for every wave, and that all have multiplied chunk c - 1, whose buffer is then refilled.
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) wrow[rb] = row_of(rb * 16 + lr);
+  for (int c = 0; c < NB - 1; ++c)
+    if (c < chunks) fill(c);
+  for (int c = 0; c < chunks; ++c) {
+    if (c + NB - 1 <= chunks) rl_wait<(NB - 2) * S::FILLS>();
+    else rl_wait<0>();  // (the last chunks: fewer are out)
+    __syncthreads();
+    if (c + NB - 1 < chunks) fill(c + NB - 1);
+    multiply(c);
+  }
+  // What is left of K, under a chunk: 32-k pieces, all requested before the first is used; rows end on a 16-byte unit, units
+  // behind the end are zeros in both operands (0 * inf).
+  const int64_t k0 = (int64_t)chunks * KC;
+  if (k0 < g.K) {
     u32x4 w[P][RB], x[P][MB];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const int64_t k = k0 + 32 * (wave + kRlWaves * p) + 8 * lg;
-      const bool in = k < g.K;
-      const int64_t kc = in ? k : 0;
+      const int64_t kc = k < g.K ? k : 0;
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) w[p][rb] = *reinterpret_cast<const u32x4*>(wrow[rb] + kc);
+      for (int rb = 0; rb < RB; ++rb) w[p][rb] = *reinterpret_cast<const u32x4*>(W + row_of(rb * 16 + lr) + kc);
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) x[p][mb] = *reinterpret_cast<const u32x4*>(xrow[mb] + kc);
+      for (int mb = 0; mb < MB; ++mb) {
+        const int64_t m = mb * 16 + lr;
+        x[p][mb] = *reinterpret_cast<const u32x4*>(X + (m < g.M ? m : g.M - 1) * g.x_rs + kc);
+      }
     }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      if (k0 + 32 * (wave + kRlWaves * p) >= g.K) break;  // (uniform over the wave)
       const bool in = k0 + 32 * (wave + kRlWaves * p) + 8 * lg < g.K;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -178,7 +199,12 @@ __global__ __launch_bounds__(64 * kRlWaves, RB == 1 ? 4 : 2) void gated_rows_lds
         for (int mb = 0; mb < MB; ++mb) acc[rb][mb] = GrMfma<T>::run(w[p][rb], x[p][mb], acc[rb][mb]);
     }
   }
-  // The waves' parts meet in LDS (the buffers are free: every chunk ends in a barrier) and are added in a fixed order.
+  // The waves' parts meet in LDS and are added in a fixed order.
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) settle(acc[rb][mb]);
+  __syncthreads();  // every wave has read the last chunk
   f32x4* meet = reinterpret_cast<f32x4*>(lds);  // [wave][block][lane]
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb)
@@ -302,6 +328,12 @@ __global__ __launch_bounds__(64 * W) void gated_rows_kernel(GatedArgs g) {
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
+      for (int mb = 0; mb < MB; ++mb) settle(acc[fb][u][mb]);
+#pragma unroll
+  for (int fb = 0; fb < FB; ++fb)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
       for (int mb = 0; mb < MB; ++mb) meet[wave][(mb * FB + fb) * 2 + u][lane] = acc[fb][u][mb];
   __syncthreads();
   // Block (token block, feature block) i goes to wave i % W, which adds the waves' parts in a fixed order.
@@ -322,11 +354,10 @@ template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t 
   using Two = integral_constant<int, 2>;
   using Four = integral_constant<int, 4>;
   using Eight = integral_constant<int, 8>;
-  auto lds = [&](auto mb, auto rb) {
-    constexpr int MB = decltype(mb)::value, RB = decltype(rb)::value;
-    const auto kern = gated_rows_lds_kernel<T, MB, RB>;
-    constexpr int bytes = 2 * RB * 16 * kRlRowBytes;
-    static_assert(bytes >= kRlWaves * RB * MB * kWave * 16, "the accumulators meet in the buffers");
+  auto lds = [&](auto rx, auto rb, auto kc, auto nb, auto waves) {
+    constexpr int RX = decltype(rx)::value, RB = decltype(rb)::value, KC = decltype(kc)::value, NB = decltype(nb)::value;
+    const auto kern = gated_rows_lds_kernel<T, RX, RB, KC, NB, decltype(waves)::value>;
+    constexpr int bytes = RowsShape<T, RX, RB, KC, NB>::LDS;
     static std::atomic<uint64_t> devices{0};
     const int rc = allow_lds(reinterpret_cast<const void*>(kern), bytes, devices, "mi355_gated_linear");
     if (rc != MI355_OK) return rc;
@@ -338,10 +369,14 @@ template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t 
     hipLaunchKernelGGL((gated_rows_kernel<T, MB, 1, W, S>), dim3((unsigned)((a.F + 15) / 16)), dim3(64 * W), 0, st, a);
     return check_launch("mi355_gated_linear");
   };
-  if (strcmp(knobs().gated_form, "direct") != 0 && a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && a.K % 8 == 0 && aligned16(a.x) && aligned16(a.w)) {
-    if (a.M <= 16) return lds(One(), One());
-    if (a.M <= 32) return lds(Two(), Two());
-    return lds(Four(), Two());
+  const bool near = a.x_rs < (1 << 30) && a.w_rs < (1 << 30);  // neighbouring rows within 32-bit byte offsets
+  if (strcmp(knobs().gated_form, "direct") != 0 && near && a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && a.K % 8 == 0 && aligned16(a.x) && aligned16(a.w)) {
+    using Half = integral_constant<int, 512>;
+    using Quarter = integral_constant<int, 256>;
+    if (a.M <= 4) return lds(Four(), One(), Half(), Four(), Four());
+    if (a.M <= 16) return lds(integral_constant<int, 16>(), Two(), Half(), integral_constant<int, 3>(), Two());
+    if (a.M <= 32) return lds(integral_constant<int, 32>(), Two(), Quarter(), integral_constant<int, 5>(), Two());
+    return lds(integral_constant<int, 64>(), Two(), Quarter(), integral_constant<int, 3>(), Two());
   }
   if (a.M <= 16) return direct(One(), Eight(), Four());
   if (a.M <= 32) return direct(Two(), Eight(), Two());
