@@ -374,7 +374,12 @@ template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t 
     using Half = integral_constant<int, 512>;
     using Quarter = integral_constant<int, 256>;
     if (a.M <= 4) return lds(Four(), One(), Half(), Four(), Four());
+    // Blocks of 8 features (x read twice as often) where those of 16 would leave half of the CUs without one: 2 * 1376 x 8192, 16
+    // and 32 tokens, 17.3 -> 12.4 and 21.0 -> 16.3 us; 2 * 2752 x 4096 11.6 and 13.2 in blocks of 16, 14.3 and 17.8 in blocks of 8.
+    const bool few = a.F <= 8 * kNumCU;
+    if (a.M <= 16 && few) return lds(integral_constant<int, 16>(), One(), Half(), integral_constant<int, 5>(), Two());
     if (a.M <= 16) return lds(integral_constant<int, 16>(), Two(), Half(), integral_constant<int, 3>(), Two());
+    if (a.M <= 32 && few) return lds(integral_constant<int, 32>(), One(), Quarter(), integral_constant<int, 6>(), Two());
     if (a.M <= 32) return lds(integral_constant<int, 32>(), Two(), Quarter(), integral_constant<int, 5>(), Two());
     return lds(integral_constant<int, 64>(), Two(), Quarter(), integral_constant<int, 3>(), Two());
   }

@@ -102,7 +102,10 @@ __global__ __launch_bounds__(kLbTile) void lb_tile_kernel(const T* __restrict__ 
     LbRaw<T, V> x[NV], dy[NV];
     float mean, rstd;
   };
-  int first[NV], skip[NV];  // first column of slab k's vector, and how many of its elements are not this lane's
+  // First column of slab k's vector, its byte offset in a row (unsigned: one register beside a row address in scalars), and how
+  // many of its elements are not this lane's.
+  int first[NV], skip[NV];
+  uint32_t at[NV];
   bool in[NV];
   LbRaw<Wt, V> gamma[NV];
 #pragma unroll
@@ -110,6 +113,7 @@ __global__ __launch_bounds__(kLbTile) void lb_tile_kernel(const T* __restrict__ 
     const int c = (k * GL + t) * V;
     in[k] = c < N;
     first[k] = c + V <= N ? c : N - V;
+    at[k] = (uint32_t)first[k] * (uint32_t)sizeof(T);
     skip[k] = TAIL && in[k] ? c - first[k] : 0;
   }
   // No branches: lanes past the row and rows past the last read what is nearest; one_row puts zeros in its place (with a
@@ -118,10 +122,12 @@ __global__ __launch_bounds__(kLbTile) void lb_tile_kernel(const T* __restrict__ 
     const int64_t rc = row < M ? row : M - 1;
     r.mean = mean[rc];
     r.rstd = rstd[rc];
+    const char *xr = reinterpret_cast<const char*>(x + rc * N), *dr = reinterpret_cast<const char*>(dy + rc * N);
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-      r.x[k].load(x + rc * N + first[k]);
-      r.dy[k].load(dy + rc * N + first[k]);
+      asm volatile("" : "+v"(at[k]));  // (else the loop carries a 64-bit pointer per slab and operand, and spills them)
+      r.x[k].load(reinterpret_cast<const T*>(xr + at[k]));
+      r.dy[k].load(reinterpret_cast<const T*>(dr + at[k]));
     }
   };
   const int64_t step = (int64_t)gridDim.x * G;
@@ -192,7 +198,8 @@ __global__ __launch_bounds__(kLbTile) void lb_tile_kernel(const T* __restrict__ 
         const float xhat = (r.x[k].get(j) - r.mean) * r.rstd;
         o.v[j] = static_cast<T>(r.rstd * (r.dy[k].get(j) * gamma[k].get(j) - m1 - xhat * m2));
       }
-      T* out = dx + row * N + first[k];
+      asm volatile("" : "+v"(at[k]));
+      T* out = reinterpret_cast<T*>(reinterpret_cast<char*>(dx + row * N) + at[k]);
       if constexpr (V == 1) {
         if (in[k]) *out = o.v[0];
       } else if (in[k] && (!TAIL || skip[k] == 0)) {
@@ -339,31 +346,34 @@ __global__ __launch_bounds__(kLbBlock) void lb_columns_kernel(const T* __restric
   }
 }
 
-// dw and db from `groups` partials of [dw | db]: 16 x 16 threads, 4 neighbouring columns and every 16th partial each.
+// dw and db from `groups` partials of [dw | db]: 32 columns per block, 8 lanes of 4 neighbouring columns by 32 threads that
+// take every 32nd partial; they meet by exchanges inside a wave (8 of them) and in LDS.
 template <typename Wt, typename S>
 __global__ __launch_bounds__(kLbBlock) void lb_finish_kernel(const S* __restrict__ partial, Wt* __restrict__ dw, Wt* __restrict__ db,
                                                             int64_t N, int groups) {
-  __shared__ S part[16][64];
-  const int q = threadIdx.x / 16, l = threadIdx.x % 16;
-  const int64_t ld_n = lb_ld(N), c0 = (int64_t)blockIdx.x * 64 + 4 * l;  // of the 2 ld_n columns [dw | db]
+  __shared__ S part[kLbBlock / kWave][32];
+  const int q = threadIdx.x / 8, l = threadIdx.x % 8;
+  const int64_t ld_n = lb_ld(N), c0 = (int64_t)blockIdx.x * 32 + 4 * l;  // of the 2 ld_n columns [dw | db]
   S s[4] = {};
   if (c0 < 2 * ld_n) {
 #pragma unroll 8
-    for (int g = q; g < groups; g += 16) {
+    for (int g = q; g < groups; g += 32) {
       const VecN<S, 4> v = ld<S, 4>(partial + (int64_t)g * 2 * ld_n + c0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[j] += v.v[j];
     }
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) part[q][4 * l + j] = s[j];
-  __syncthreads();
-  const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  const int64_t col = c < ld_n ? c : c - ld_n;
-  if (threadIdx.x >= 64 || c >= 2 * ld_n || col >= N) return;
-  S sum = 0;
+  for (int j = 0; j < 4; ++j) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sum += part[i][threadIdx.x];
+    for (int d = 8; d < kWave; d *= 2) s[j] += __shfl_xor(s[j], d, kWave);
+    if (threadIdx.x % kWave < 8) part[threadIdx.x / kWave][4 * l + j] = s[j];
+  }
+  __syncthreads();
+  const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  const int64_t col = c < ld_n ? c : c - ld_n;
+  if (threadIdx.x >= 32 || c >= 2 * ld_n || col >= N) return;
+  const S sum = (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
   Wt* out = c < ld_n ? dw : db;
   if (out) out[col] = static_cast<Wt>(sum);
 }
@@ -442,7 +452,7 @@ static int run_lb_tile(const LbTile& p, const T* dy, const T* x, const float* me
   }
 #undef MI355_LB_TILE
   if (rc != MI355_OK || partial == nullptr) return rc;
-  hipLaunchKernelGGL((lb_finish_kernel<Wt, float>), dim3((unsigned)((2 * lb_ld(N) + 63) / 64)), dim3(kLbBlock), 0, st, partial, dw, db, N, (int)blocks);
+  hipLaunchKernelGGL((lb_finish_kernel<Wt, float>), dim3((unsigned)((2 * lb_ld(N) + 31) / 32)), dim3(kLbBlock), 0, st, partial, dw, db, N, (int)blocks);
   return check_launch("mi355_layer_norm_backward");
 }
 
@@ -466,7 +476,7 @@ static int run_lb(const void* dyv, const void* xv, const void* mv, const void* r
   hipLaunchKernelGGL((lb_columns_kernel<T, Wt, S>), dim3((unsigned)((N + kLbBlock - 1) / kLbBlock), (unsigned)p.groups), dim3(kLbBlock), 0, st, dy,
                      x, mean, rstd, w, sums, static_cast<T*>(dxv), partial, M, N, p.rows_per_group);
   if (partial)
-    hipLaunchKernelGGL((lb_finish_kernel<Wt, S>), dim3((unsigned)((2 * lb_ld(N) + 63) / 64)), dim3(kLbBlock), 0, st, partial,
+    hipLaunchKernelGGL((lb_finish_kernel<Wt, S>), dim3((unsigned)((2 * lb_ld(N) + 31) / 32)), dim3(kLbBlock), 0, st, partial,
                        static_cast<Wt*>(dwv), static_cast<Wt*>(dbv), N, (int)p.groups);
   return check_launch("mi355_layer_norm_backward");
 }
