@@ -120,7 +120,8 @@ TRAIN_SIGNATURES = {
         c_int,
         [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_void_p],
     ),
-    "mi355_gated_act": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p]),
+    "mi355_pad_rows": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p]),
+    "mi355_gated_act": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_void_p]),
     "mi355_gated_linear_backward_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int]),
     "mi355_gated_linear_backward": (
         c_int,

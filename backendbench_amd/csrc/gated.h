@@ -3,7 +3,7 @@
 #include <type_traits>
 
 #include "../../include/mi355_train.h"
-#include "common.h"
+#include "elementwise.h"  // VecN
 
 namespace mi355 {
 
@@ -61,6 +61,24 @@ template <int ACT, typename A, typename F> __device__ __forceinline__ F gate_gra
 // The arithmetic for results of type T.
 template <typename T> using GateMath = std::conditional_t<sizeof(T) == 2, GateHalf, typename OpMath<T>::type>;
 
+// 16 bytes at an address that is only a multiple of an element's size.
+template <int B> struct AnyVec;
+template <> struct AnyVec<2> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct AnyVec<4> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct AnyVec<8> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(8))); };
+// The V = 16 / sizeof(T) elements from p on, of which `count` are there (the rest become zeros).
+template <typename T, int V = 16 / sizeof(T)> __device__ __forceinline__ VecN<T, V> load_some(const T* p, int64_t count) {
+  VecN<T, V> v{};
+  if (count >= V) {
+    v = __builtin_bit_cast(decltype(v), __builtin_nontemporal_load(reinterpret_cast<const typename AnyVec<sizeof(T)>::type*>(p)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (j < count) v.v[j] = p[j];
+  }
+  return v;
+}
+
 // body(ACT) with an integral constant.
 template <typename Body> static int dispatch_act(int act, const char* name, Body body) {
   switch (act) {
@@ -85,8 +103,9 @@ bool gated_x16_takes(const GatedArgs& a);
 int launch_gated_x16(const GatedArgs& a, hipStream_t st);
 // gemm.hip: 128 rows by 64 features per workgroup; K % 64 == 0, 16-byte aligned rows
 int launch_gated_small2(const GatedArgs& a, hipStream_t st);
-// gated_rows.hip: at most kGatedRows rows, any K, strides and alignment
-constexpr int64_t kGatedRows = 64;
+// gated_rows.hip: at most this many rows, aligned or at any address
+constexpr int64_t kGatedRows = 64, kGatedRowsAnywhere = 4;
+bool gated_rows_takes(const GatedArgs& a);
 int launch_gated_rows(const GatedArgs& a, hipStream_t st);
 
 }  // namespace mi355

@@ -13,26 +13,10 @@ namespace mi355 {
 
 constexpr int kGbTile = 64;
 
-// 16 bytes at an address that is only a multiple of an element's size.
-template <int B> struct GbAny;
-template <> struct GbAny<2> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2))); };
-template <> struct GbAny<4> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4))); };
-template <> struct GbAny<8> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(8))); };
-// The V = 16 / sizeof(T) elements from p on, of which `count` are there (the rest become zeros).
-template <typename T, int V = 16 / sizeof(T)> __device__ __forceinline__ VecN<T, V> gb_load(const T* p, int64_t count) {
-  VecN<T, V> v{};
-  if (count >= V) {
-    v = __builtin_bit_cast(decltype(v), __builtin_nontemporal_load(reinterpret_cast<const typename GbAny<sizeof(T)>::type*>(p)));
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (j < count) v.v[j] = p[j];
-  }
-  return v;
-}
+// The first `count` elements of v.
 template <typename T, int V> __device__ __forceinline__ void gb_store(T* p, int64_t count, const VecN<T, V>& v) {
   if (count >= V) {
-    *reinterpret_cast<typename GbAny<sizeof(T)>::type*>(p) = __builtin_bit_cast(u32x4, v);
+    *reinterpret_cast<typename AnyVec<sizeof(T)>::type*>(p) = __builtin_bit_cast(u32x4, v);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -59,9 +43,9 @@ __global__ __launch_bounds__(256) void gated_dpre_kernel(const T* __restrict__ d
     const int e = (threadIdx.x + 256 * i) * V;
     const int64_t m = m0 + e / kGbTile, f = f0 + e % kGbTile;
     const int64_t there = m < M && e < TM * kGbTile ? F - f : 0;
-    gv[i] = gb_load(pre + m * 2 * F + f, there);
-    uv[i] = gb_load(pre + m * 2 * F + F + f, there);
-    dv[i] = gb_load(dh + m * F + f, there);
+    gv[i] = load_some(pre + m * 2 * F + f, there);
+    uv[i] = load_some(pre + m * 2 * F + F + f, there);
+    dv[i] = load_some(dh + m * F + f, there);
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -123,7 +107,7 @@ __global__ __launch_bounds__(256) void turn_pad_kernel(const B* __restrict__ src
   for (int i = 0; i < PER; ++i) {
     const int e = (threadIdx.x + 256 * i) * V;
     const int64_t r = r0 + e / kGbTile, c = c0 + e % kGbTile;
-    v[i] = gb_load(src + r * rs + c, r < R ? C - c : 0);
+    v[i] = load_some(src + r * rs + c, r < R ? C - c : 0);
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {

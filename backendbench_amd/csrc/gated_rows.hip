@@ -223,63 +223,41 @@ __global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_
   }
 }
 
-// Rows at any address: fragments straight from global memory, a workgroup owns FB x 16 features, gate and up, and its W waves
-// take turns along K, 32 S elements at a time, each with its next step's loads in flight while it computes.
-// Operand fragment of a 32-k piece: lane l holds row l % 16, k = 8 (l / 16) .. + 7 of it.  With the weight as the first
-// operand, element e of an accumulator in lane l is feature 4 (l / 16) + e of token l % 16.
-template <typename T, int MB, int FB, int W, int S>
-__global__ __launch_bounds__(64 * W) void gated_rows_kernel(GatedArgs g) {
-  __shared__ f32x4 meet[W][MB * FB * 2][kWave];
+// Rows at any address, up to 16 tokens: fragments straight from global memory, eight waves to a workgroup of 16 features, gate
+// and up; the waves take turns along K, 128 elements at a time, each with its next step's loads in flight while it computes.
+// 1.8 TB/s of the weight at K = 5001 (55 us for 2 * 5001 rows and one token): the misaligned 64-byte requests are the bound.
+// A copy into aligned rows in front of the other kernel costs as much for one token and less from five on.
+constexpr int kGrSteps = 4;  // 32-k pieces of a step
+
+template <typename T>
+__global__ __launch_bounds__(64 * kRlWaves) void gated_rows_kernel(GatedArgs g) {
+  __shared__ f32x4 meet[kRlWaves][2][kWave];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lr = lane & 15, lg = lane >> 4;
-  const int64_t f0 = (int64_t)blockIdx.x * (16 * FB);
-  const T* wrow[FB][2];
-  const T* xrow[MB];
-#pragma unroll
-  for (int fb = 0; fb < FB; ++fb) {
-    int64_t f = f0 + fb * 16 + lr;
-    f = f < g.F ? f : g.F - 1;  // features past the last are computed on its row and not stored
-    wrow[fb][0] = static_cast<const T*>(g.w) + f * g.w_rs;
-    wrow[fb][1] = static_cast<const T*>(g.w) + (g.F + f) * g.w_rs;
-  }
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    const int64_t m = mb * 16 + lr;
-    xrow[mb] = static_cast<const T*>(g.x) + (m < g.M ? m : g.M - 1) * g.x_rs;
-  }
+  const int64_t f0 = (int64_t)blockIdx.x * 16;
+  const int64_t f = f0 + lr < g.F ? f0 + lr : g.F - 1;  // features past the last are computed on its row and not stored
+  const T* wrow[2] = {static_cast<const T*>(g.w) + f * g.w_rs, static_cast<const T*>(g.w) + (g.F + f) * g.w_rs};
+  const T* xrow = static_cast<const T*>(g.x) + (lr < g.M ? lr : g.M - 1) * g.x_rs;
   struct Step {
-    u32x4 w[FB][2][S], x[MB][S];
+    u32x4 w[2][kGrSteps], x[kGrSteps];
   };
   auto fetch = [&](int64_t k, Step& s) {
 #pragma unroll
-    for (int p = 0; p < S; ++p) {
+    for (int p = 0; p < kGrSteps; ++p) {
       const int64_t c = k + 32 * p + 8 * lg;
 #pragma unroll
-      for (int fb = 0; fb < FB; ++fb)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) s.w[fb][u][p] = __builtin_nontemporal_load(reinterpret_cast<const gr_any*>(wrow[fb][u] + c));
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) s.x[mb][p] = *reinterpret_cast<const gr_any*>(xrow[mb] + c);
+      for (int u = 0; u < 2; ++u) s.w[u][p] = __builtin_nontemporal_load(reinterpret_cast<const gr_any*>(wrow[u] + c));
+      s.x[p] = *reinterpret_cast<const gr_any*>(xrow + c);
     }
   };
-  f32x4 acc[FB][2][MB];
-#pragma unroll
-  for (int fb = 0; fb < FB; ++fb)
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) acc[fb][u][mb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
   auto multiply = [&](const Step& s) {
 #pragma unroll
-    for (int p = 0; p < S; ++p)
+    for (int p = 0; p < kGrSteps; ++p)
 #pragma unroll
-      for (int fb = 0; fb < FB; ++fb)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int mb = 0; mb < MB; ++mb) acc[fb][u][mb] = GrMfma<T>::run(s.w[fb][u][p], s.x[mb][p], acc[fb][u][mb]);
+      for (int u = 0; u < 2; ++u) acc[u] = GrMfma<T>::run(s.w[u][p], s.x[p], acc[u]);
   };
-  constexpr int64_t KS = 32 * S, ROUND = KS * W;
+  constexpr int64_t KS = 32 * kGrSteps, ROUND = KS * kRlWaves;
   const int64_t whole = g.K / KS * KS;  // whole steps
   int64_t k = wave * KS;
   if (k < whole) {
@@ -298,54 +276,33 @@ __global__ __launch_bounds__(64 * W) void gated_rows_kernel(GatedArgs g) {
   }
   // What is left of K, 32 elements per wave: eight elements of a row at a time when they are there, else one by one, zeros
   // behind the end (in both operands: 0 * inf).
-  for (int64_t k1 = whole + 32 * wave; k1 < g.K; k1 += 32 * W) {
+  for (int64_t k1 = whole + 32 * wave; k1 < g.K; k1 += 32 * kRlWaves) {
     const int64_t c = k1 + 8 * lg;
-    auto piece = [&](const T* row) {
-      u32x4 v = {0u, 0u, 0u, 0u};
-      if (c + 8 <= g.K) {
-        v = *reinterpret_cast<const gr_any*>(row + c);
-      } else {
+    const u32x4 xv = __builtin_bit_cast(u32x4, load_some(reinterpret_cast<const uint16_t*>(xrow) + c, g.K - c));
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c + j < g.K) v[j >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, row[c + j]) << (16 * (j & 1));
-      }
-      return v;
-    };
-    u32x4 xv[MB];
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb) xv[mb] = piece(xrow[mb]);
-#pragma unroll
-    for (int fb = 0; fb < FB; ++fb)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const u32x4 wv = piece(wrow[fb][u]);
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) acc[fb][u][mb] = GrMfma<T>::run(wv, xv[mb], acc[fb][u][mb]);
-      }
-  }
-#pragma unroll
-  for (int fb = 0; fb < FB; ++fb)
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) settle(acc[fb][u][mb]);
-#pragma unroll
-  for (int fb = 0; fb < FB; ++fb)
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) meet[wave][(mb * FB + fb) * 2 + u][lane] = acc[fb][u][mb];
-  __syncthreads();
-  // Block (token block, feature block) i goes to wave i % W, which adds the waves' parts in a fixed order.
-  for (int i = wave; i < MB * FB; i += W) {
-    f32x4 gv = meet[0][2 * i][lane], uv = meet[0][2 * i + 1][lane];
-#pragma unroll
-    for (int q = 1; q < W; ++q) {
-      gv += meet[q][2 * i][lane];
-      uv += meet[q][2 * i + 1][lane];
+    for (int u = 0; u < 2; ++u) {
+      const u32x4 wv = __builtin_bit_cast(u32x4, load_some(reinterpret_cast<const uint16_t*>(wrow[u]) + c, g.K - c));
+      acc[u] = GrMfma<T>::run(wv, xv, acc[u]);
     }
-    store_rows<T>(g, (i / FB) * 16 + lr, f0 + (i % FB) * 16 + 4 * lg, gv, uv);
   }
+#pragma unroll
+  for (int u = 0; u < 2; ++u) settle(acc[u]);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) meet[wave][u][lane] = acc[u];
+  __syncthreads();
+  if (wave != 0) return;
+  f32x4 gv = meet[0][0][lane], uv = meet[0][1][lane];  // the waves' parts, in a fixed order
+#pragma unroll
+  for (int q = 1; q < kRlWaves; ++q) {
+    gv += meet[q][0][lane];
+    uv += meet[q][1][lane];
+  }
+  store_rows<T>(g, lr, f0 + 4 * lg, gv, uv);
+}
+
+// Rows on 16-byte boundaries, of whole 16-byte units, and neighbours within a request's 32-bit byte offset.
+static bool rows_aligned(const GatedArgs& a) {
+  return a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && a.K % 8 == 0 && aligned16(a.x) && aligned16(a.w) && a.x_rs < (1 << 30) && a.w_rs < (1 << 30);
 }
 
 template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t st) {
@@ -353,7 +310,6 @@ template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t 
   using One = integral_constant<int, 1>;
   using Two = integral_constant<int, 2>;
   using Four = integral_constant<int, 4>;
-  using Eight = integral_constant<int, 8>;
   auto lds = [&](auto rx, auto rb, auto kc, auto nb, auto waves) {
     constexpr int RX = decltype(rx)::value, RB = decltype(rb)::value, KC = decltype(kc)::value, NB = decltype(nb)::value;
     const auto kern = gated_rows_lds_kernel<T, RX, RB, KC, NB, decltype(waves)::value>;
@@ -364,13 +320,7 @@ template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t 
     hipLaunchKernelGGL(kern, dim3((unsigned)((a.F + 8 * RB - 1) / (8 * RB))), dim3(64 * kRlWaves), bytes, st, a);
     return check_launch("mi355_gated_linear");
   };
-  auto direct = [&](auto mb, auto w, auto s) {
-    constexpr int MB = decltype(mb)::value, W = decltype(w)::value, S = decltype(s)::value;
-    hipLaunchKernelGGL((gated_rows_kernel<T, MB, 1, W, S>), dim3((unsigned)((a.F + 15) / 16)), dim3(64 * W), 0, st, a);
-    return check_launch("mi355_gated_linear");
-  };
-  const bool near = a.x_rs < (1 << 30) && a.w_rs < (1 << 30);  // neighbouring rows within 32-bit byte offsets
-  if (strcmp(knobs().gated_form, "direct") != 0 && near && a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && a.K % 8 == 0 && aligned16(a.x) && aligned16(a.w)) {
+  if (strcmp(knobs().gated_form, "direct") != 0 && rows_aligned(a)) {
     using Half = integral_constant<int, 512>;
     using Quarter = integral_constant<int, 256>;
     if (a.M <= 4) return lds(Four(), One(), Half(), Four(), Four());
@@ -383,10 +333,11 @@ template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t 
     if (a.M <= 32) return lds(integral_constant<int, 32>(), Two(), Quarter(), integral_constant<int, 5>(), Two());
     return lds(integral_constant<int, 64>(), Two(), Quarter(), integral_constant<int, 3>(), Two());
   }
-  if (a.M <= 16) return direct(One(), Eight(), Four());
-  if (a.M <= 32) return direct(Two(), Eight(), Two());
-  return direct(Four(), Eight(), Two());
+  hipLaunchKernelGGL((gated_rows_kernel<T>), dim3((unsigned)((a.F + 15) / 16)), dim3(64 * kRlWaves), 0, st, a);
+  return check_launch("mi355_gated_linear");
 }
+
+bool gated_rows_takes(const GatedArgs& a) { return a.F < (1 << 25) && a.M <= (rows_aligned(a) ? kGatedRows : kGatedRowsAnywhere); }
 
 int launch_gated_rows(const GatedArgs& a, hipStream_t st) {
   return a.dtype == MI355_BF16 ? run_gated_rows<bf16_t>(a, st) : run_gated_rows<f16_t>(a, st);

@@ -99,9 +99,9 @@ static int run_gated_x16(const GatedArgs& a, hipStream_t st) {
 }
 
 bool gated_x16_takes(const GatedArgs& a) {
-  // 32-bit byte offsets: up to 256 rows of x and the whole gate half of the weight plus a tile.
-  return a.K % 128 == 0 && a.K >= 256 && a.x_rs < (1 << 22) && (a.F + 128) * a.w_rs < (int64_t(1) << 31) - 4096 &&
-         ((a.M + 255) / 256) * ((a.F + 127) / 128) < (int64_t(1) << 31);
+  // 32-bit byte offsets over up to 256 rows of either operand; fewer than 2^32 threads
+  return a.K % 128 == 0 && a.K >= 256 && a.x_rs < (1 << 22) && a.w_rs < (1 << 22) &&
+         ((a.M + 255) / 256) * ((a.F + 127) / 128) < (int64_t(1) << 24);
 }
 
 int launch_gated_x16(const GatedArgs& a, hipStream_t st) {

@@ -1,5 +1,6 @@
-// The tile of mm / addmm on v_mfma_f32_16x16x32 (kernels: gemm_x16.hip; the gated projection: gated_x16.hip): 256x256 tiles, four waves of 128x128 (8 x 8 blocks of 16x16, 256
-// fp32 accumulators per lane), bf16 / f16, K % 128 == 0, K >= 256, a K-contiguous, b K-contiguous or row-major.
+// The tile of mm / addmm (kernels: gemm_x16.hip) and of the gated projection (gated_x16.hip) on v_mfma_f32_16x16x32:
+// 256x256, four waves of 128x128 (8 x 8 blocks of 16x16, 256 fp32 accumulators per lane), bf16 / f16, K % 128 == 0,
+// K >= 256, a K-contiguous, b K-contiguous or row-major.
 //
 // Why a second form of the four-wave kernel.  On real operand data the GEMM is bound by the power
 // envelope, not by issue slots: the clock falls when a kernel does more per cycle.  The MFMA stream
@@ -461,6 +462,7 @@ __device__ __forceinline__ void x16_tile(const GemmArgs& g, unsigned char* lds, 
   const unsigned char* b_base = b_start(PERSIST ? col0(ptn) : bn);
   const int64_t a_step = 128;                                   // bytes per 64-k stage
   const int64_t b_step = B_NN ? (int64_t)128 * g.ldb : 128;
+  const int64_t b_half = GATED ? (int64_t)g.N * g.ldb * 2 : 0;  // from the first B set's rows to the second's
   uint32_t a_off[2][4], b_off[2][4];
 #pragma unroll
   for (int x = 0; x < 2; ++x)
@@ -477,10 +479,10 @@ __device__ __forceinline__ void x16_tile(const GemmArgs& g, unsigned char* lds, 
         int gn = bn + (cc >> 6) * WCOLS + x * HCOLS + (cc & 63);
         gn = gn < g.N ? gn : 0;
         b_off[x][i] = ((uint32_t)k * (uint32_t)g.ldb + (uint32_t)gn) * 2u + (uint32_t)(kXBias - 1024 * i);
-      } else if constexpr (GATED) {  // x = 0: the gate rows, 1: the up rows of the same features
+      } else if constexpr (GATED) {  // x = 0: the gate rows, 1: the up rows of the same features, b_half bytes further
         int ln = (r >> 6) * 64 + (r & 63);
         ln = bn + ln < g.N ? ln : g.N - 1 - bn;
-        b_off[x][i] = ((uint32_t)(x * g.N + ln) * (uint32_t)g.ldb + (uint32_t)c * 8u) * 2u + (uint32_t)(kXBias - 1024 * i);
+        b_off[x][i] = ((uint32_t)ln * (uint32_t)g.ldb + (uint32_t)c * 8u) * 2u + (uint32_t)(kXBias - 1024 * i);
       } else {
         int ln = (r >> 6) * WCOLS + x * HCOLS + (r & 63);
         ln = bn + ln < g.N ? ln : g.N - 1 - bn;
@@ -608,10 +610,10 @@ __device__ __forceinline__ void x16_tile(const GemmArgs& g, unsigned char* lds, 
     if constexpr ((HH & 1) == 0) {
       // first half of the stage: (B0, A_H) then (B0, A_(1-H)); pair t + 1 = {A_(1-H)(S), B1(S)}
       quadrant(std::integral_constant<int, H>{}, I0{}, std::true_type{}, LA{}, XRc{}, FILL_, pair, m0a, a_off[XF], fa);
-      quadrant(std::integral_constant<int, 1 - H>{}, I0{}, std::true_type{}, LB{}, I1{}, FILL_, pair, m0b, b_off[YF], fb);
+      quadrant(std::integral_constant<int, 1 - H>{}, I0{}, std::true_type{}, LB{}, I1{}, FILL_, pair, m0b, b_off[YF], YF ? fb + b_half : fb);
     } else {
       // second half: (B1, A_(1-H)) then (B1, A_H); pair t + 1 = {A_h'(S+1), B0(S+1)}, h' = 1 - H
-      quadrant(std::integral_constant<int, 1 - H>{}, I1{}, std::false_type{}, LB{}, I0{}, FILL_, pair, m0b, b_off[YF], fb);
+      quadrant(std::integral_constant<int, 1 - H>{}, I1{}, std::false_type{}, LB{}, I0{}, FILL_, pair, m0b, b_off[YF], YF ? fb + b_half : fb);
       quadrant(std::integral_constant<int, H>{}, I1{}, std::false_type{}, LA{}, XRc{}, FILL_, pair, m0a, a_off[XF], fa);
     }
 #ifdef MI355_GEMM_TRACE
@@ -670,10 +672,10 @@ __device__ __forceinline__ void x16_tile(const GemmArgs& g, unsigned char* lds, 
     fill_i(I2{}, a_off[x], a_base + s * a_step);
     fill_i(I3{}, a_off[x], a_base + s * a_step);
     x16_set_m0(m0a + (uint32_t)kXSub);
-    fill_i(I0{}, b_off[second], b_base + s * b_step);
-    fill_i(I1{}, b_off[second], b_base + s * b_step);
-    fill_i(I2{}, b_off[second], b_base + s * b_step);
-    fill_i(I3{}, b_off[second], b_base + s * b_step);
+    fill_i(I0{}, b_off[second], b_base + s * b_step + second * b_half);
+    fill_i(I1{}, b_off[second], b_base + s * b_step + second * b_half);
+    fill_i(I2{}, b_off[second], b_base + s * b_step + second * b_half);
+    fill_i(I3{}, b_off[second], b_base + s * b_step + second * b_half);
   }
   if constexpr (PERSIST) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // all five: the first tile's waits assume what later tiles find
   else asm volatile("s_waitcnt vmcnt(24)" ::: "memory");

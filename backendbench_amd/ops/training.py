@@ -11,7 +11,7 @@ from .. import _lib
 from ._common import cast, copy_into, dense, launch, new_dense, new_result, on_gpu, prod, try_launch
 from .elementwise import _store_result as store_result
 from .elementwise import tuple_out_variant
-from .matmul import _gemm, _gemm_f32out
+from .matmul import _gemm
 
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16, torch.float64)
 _HALF = (torch.bfloat16, torch.float16)
@@ -142,33 +142,28 @@ def gated_linear(input, weight, activation="silu", save_pre=False):
     return _gated_linear(input, weight, _ACTIVATIONS[activation], save_pre)
 
 
-_PAD_ROWS = 64  # more rows than this are worth a zero-padded copy of a weight whose rows the kernels cannot take
-
-
 def _rows_of(t):
     """`t` [R, K] itself when its rows are unit-stride and do not overlap, else a dense copy."""
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else dense(t)
 
 
-def _gated_fused(x, weight, h, pre, act):
-    """The one-kernel form on x [M, K]; False when there is none for these operands (nothing was launched)."""
+def _padded(t, columns):
+    """A copy of `t` [R, K] in aligned rows of `columns` elements, zeros behind the K that are there (a product's terms 0 * 0)."""
+    out = new_dense((t.shape[0], columns), t.dtype, t.device)
+    launch("mi355_pad_rows", t.data_ptr(), t.stride(0), t.shape[0], t.shape[1], out.data_ptr(), columns, t.element_size())
+    return out
+
+
+def _gated_half(x, weight, h, pre, act):
+    """bf16 / f16: one kernel, on padded copies of the operands where no kernel takes their rows as they are."""
     M, K = x.shape
     F = weight.shape[0] // 2
     code = _lib.DTYPE[x.dtype]
-    weight = _rows_of(weight)
-    if try_launch("mi355_gated_linear", x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), h.data_ptr(), _ptr(pre), M, F, K,
-                  act, code):
-        return True
-    if M <= _PAD_ROWS:
-        return False
-    # copied once into aligned rows of a multiple of 128 (exact: the pad adds 0 * 0 terms)
-    Kp = max((K + 127) // 128 * 128, 256)
-    both = new_dense((M + 2 * F, Kp), x.dtype, x.device)
-    copy_into(both[:M, :K], x)
-    copy_into(both[M:, :K], weight)
-    if Kp > K:
-        both[:, K:].zero_()
-    return try_launch("mi355_gated_linear", both.data_ptr(), Kp, both[M:].data_ptr(), Kp, h.data_ptr(), _ptr(pre), M, F, Kp, act, code)
+    if not try_launch("mi355_gated_linear", x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), h.data_ptr(), _ptr(pre), M, F,
+                      K, act, code):
+        Kp = max((K + 127) // 128 * 128, 256)
+        x, weight = _padded(x, Kp), _padded(weight, Kp)
+        launch("mi355_gated_linear", x.data_ptr(), Kp, weight.data_ptr(), Kp, h.data_ptr(), _ptr(pre), M, F, Kp, act, code)
 
 
 @on_gpu
@@ -180,19 +175,18 @@ def _gated_linear(input, weight, act, save_pre):
         h = torch.zeros((*lead, F), dtype=dtype, device=device)
         return (h, torch.zeros((*lead, 2 * F), dtype=dtype, device=device)) if save_pre else h
     h = new_dense((*lead, F), dtype, device)
-    pre = new_dense((*lead, 2 * F), dtype, device) if save_pre and dtype in _HALF else None
     x = _rows_of(input) if input.dim() == 2 else dense(input).view(M, K)
+    weight = _rows_of(weight)
     if dtype in _HALF:
-        if _gated_fused(x, weight, h, pre, act):
-            return (h, pre) if save_pre else h
-        wide, saved = _gemm_f32out(x, weight.t(), None, 1.0, 0.0), pre
-    else:
-        wide, saved = _gemm(x, weight.t(), None, 1.0, 0.0), None
-        if save_pre:
-            pre = wide.view(*lead, 2 * F)
-    launch("mi355_gated_act", wide.data_ptr(), _lib.dtype_code(wide.dtype), h.data_ptr(),
-           _ptr(saved), _lib.dtype_code(dtype), M, F, act)
-    return (h, pre) if save_pre else h
+        pre = new_dense((*lead, 2 * F), dtype, device) if save_pre else None
+        _gated_half(x, weight, h, pre, act)
+        return (h, pre) if save_pre else h
+    if dtype == torch.float32 and M * F >= 1024 and (K % 16 or x.data_ptr() % 16 or weight.data_ptr() % 16):
+        Kp = (K + 63) // 64 * 64  # rows the fp32 matrix instructions' kernel takes
+        x, weight = _padded(x, Kp), _padded(weight, Kp)
+    pre = _gemm(x, weight.t(), None, 1.0, 0.0)
+    launch("mi355_gated_act", pre.data_ptr(), h.data_ptr(), _lib.DTYPE[dtype], M, F, act)
+    return (h, pre.view(*lead, 2 * F)) if save_pre else h
 
 
 def gated_linear_backward(grad_out, input, weight, pre, activation="silu", output_mask=(True, True)):

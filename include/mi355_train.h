@@ -38,18 +38,21 @@ typedef enum mi355_activation {
 
 /* h = act(x Wg^T) * (x Wu^T) in one kernel: x [M][K] with rows x_rs apart, weight [2F][K] = [Wg; Wu] with rows w_rs
  * apart, both unit-stride along K; h [M][F] dense; pre (may be NULL) receives the pre-activations [M][2F], dense.  All of
- * `dtype`.  Products accumulate in fp32; the activation takes the unrounded sums.  For f16 / bf16: up to 64 rows
- * with any K, strides and alignment; more with 16-byte aligned rows of K % 128 == 0, K >= 256 (K % 64 == 0
- * where (M / 128) (F / 64) tiles are at most 512).  Otherwise MI355_ERR_UNSUPPORTED with nothing launched (a product and mi355_gated_act do it). */
+ * `dtype`, f16 or bf16.  Products accumulate in fp32; the activation takes the unrounded sums.  Up to 4 rows with any K,
+ * strides and alignment; up to 64 with 16-byte aligned rows and K % 8 == 0; more with such rows and K % 128 == 0, or
+ * K % 64 == 0 and at most 512 tiles of 128 rows by 64 features.  Otherwise MI355_ERR_UNSUPPORTED with nothing launched
+ * (mi355_pad_rows brings any operands into a form that is taken). */
 int mi355_gated_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, void* h, void* pre, int64_t M, int64_t F,
                        int64_t K, int act, int dtype, void* stream);
 
-/* h[m][f] = act(pre[m][f]) * pre[m][F + f] from dense pre [M][2F]; pre_out (may be NULL) receives pre rounded to
- * `dtype`.  pre_dtype: dtype, or f32 for f16 / bf16 results. */
-int mi355_gated_act(const void* pre, int pre_dtype, void* h, void* pre_out, int dtype, int64_t M, int64_t F, int act,
-                    void* stream);
+/* dst [R][ld] = src [R][C] with rows src_rs apart at any alignment, columns C .. ld - 1 zeros, elements of 2 or 4 bytes moved
+ * as bits; dst and its rows start on 16-byte boundaries.  It brings x and weight into rows that the kernels take. */
+int mi355_pad_rows(const void* src, int64_t src_rs, int64_t R, int64_t C, void* dst, int64_t ld, int element_size, void* stream);
 
-/* Its gradients: dpre = [dh * up * act'(gate) | dh * act(gate)] with gate = pre[m][f], up = pre[m][F + f], rounded once to
+/* h[m][f] = act(pre[m][f]) * pre[m][F + f] from dense pre [M][2F], f32 or f64: the activation behind a product. */
+int mi355_gated_act(const void* pre, void* h, int dtype, int64_t M, int64_t F, int act, void* stream);
+
+/* The gated projection's gradients: dpre = [dh * up * act'(gate) | dh * act(gate)] with gate = pre[m][f], up = pre[m][F + f], rounded once to
  * `dtype` (f32, f16, bf16, f64), then dx [M][K] = dpre W and dweight [2F][K] = dpre^T x, accumulated in fp32 (fp64).  dh
  * [M][F], pre [M][2F], dx and dweight are dense; x and weight have rows x_rs and w_rs apart.  dx or dweight may be NULL.
  * The workspace (16-byte aligned, contents undefined before and after; not shared by calls that may overlap in time)

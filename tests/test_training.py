@@ -144,18 +144,25 @@ def test_c_entry_points_check_their_arguments():
     assert ln(None, None, _lib.F32, None, None, None, _lib.F32, p, None, None, 0, 8, None, 0, None) == 0
     assert lib.mi355_layer_norm_backward_workspace_bytes(0, 8, _lib.F32) == 0
     act = lib.mi355_gated_act
-    refused(act(p, _lib.F32, p, None, _lib.F32, 4, 8, 3, None), b"activation")
-    refused(act(None, _lib.F32, p, None, _lib.F32, 4, 8, 0, None), b"NULL")
-    refused(act(p, _lib.F16, p, None, _lib.F32, 4, 8, 0, None), b"no kernel")
-    refused(act(p, _lib.I32, p, None, _lib.I32, 4, 8, 0, None), b"unsupported")
-    refused(act(p, _lib.F32, p, None, _lib.F32, -4, 8, 0, None), b"negative")
+    refused(act(p, p, _lib.F32, 4, 8, 3, None), b"activation")
+    refused(act(None, p, _lib.F32, 4, 8, 0, None), b"NULL")
+    refused(act(p, p, _lib.BF16, 4, 8, 0, None), b"unsupported")
+    refused(act(p, p, _lib.F32, -4, 8, 0, None), b"negative")
+    pad = lib.mi355_pad_rows
+    refused(pad(p, 8, 4, 8, p, 12, 2, None), b"rows of 12")
+    refused(pad(p, 8, 4, 8, p, 16, 8, None), b"of 8 bytes")
+    refused(pad(p, 7, 4, 8, p, 16, 2, None), b"extents")
+    refused(pad(p, 16, 4, 16, p, 8, 2, None), b"extents")
+    refused(pad(p, 8, 4, 8, p + 8, 16, 2, None), b"misaligned")
+    refused(pad(None, 8, 4, 8, p, 16, 2, None), b"NULL")
+    assert pad(None, 8, 0, 8, None, 16, 2, None) == 0
     fwd = lib.mi355_gated_linear
     refused(fwd(p, 64, p, 64, p, None, 4, 8, 64, 3, _lib.BF16, None), b"activation")
     refused(fwd(None, 64, p, 64, p, None, 4, 8, 64, 0, _lib.BF16, None), b"NULL")
     refused(fwd(p, 63, p, 64, p, None, 4, 8, 64, 0, _lib.BF16, None), b"overlap")
     refused(fwd(p, 64, p, 0, p, None, 4, 8, 64, 0, _lib.BF16, None), b"overlap")
     refused(fwd(p, 64, p, 64, p, None, 4, -8, 64, 0, _lib.BF16, None), b"negative")
-    for rows, K, dtype in ((4, 64, _lib.F32), (4, 64, _lib.F64), (4, 64, _lib.I8), (65, 63, _lib.BF16), (65, 72, _lib.F16), (4, 0, _lib.BF16)):
+    for rows, K, dtype in ((4, 64, _lib.F32), (4, 64, _lib.F64), (4, 64, _lib.I8), (65, 63, _lib.BF16), (65, 72, _lib.F16), (5, 63, _lib.BF16), (4, 0, _lib.BF16)):
         assert fwd(p, K, p, K, p, None, rows, 8, K, 0, dtype, None) == -2     # unsupported, nothing launched
     assert fwd(None, 64, None, 64, None, None, 0, 8, 64, 0, _lib.BF16, None) == 0
     back, size = lib.mi355_gated_linear_backward, lib.mi355_gated_linear_backward_workspace_bytes

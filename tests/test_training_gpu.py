@@ -261,7 +261,7 @@ def gated_form():
 
 @pytest.mark.parametrize("form,M,K,F", [
     ("rows", 1, 2048, 40), ("rows", 16, 1016, 24), ("rows", 17, 2056, 23), ("rows", 64, 4104, 129), ("rows", 33, 8, 1), ("rows", 5, 5120, 8),
-    ("direct", 1, 2048, 40), ("direct", 40, 1000, 129), ("direct", 20, 77, 9),
+    ("direct", 1, 2048, 40), ("direct", 16, 1000, 129), ("direct", 4, 77, 9), ("direct", 3, 1331, 33),
     ("tile128", 1, 64, 1), ("tile128", 130, 128, 70), ("tile128", 64, 192, 64), ("tile128", 300, 256, 129), ("tile128", 257, 448, 200),
     ("tile128", 128, 1024, 336),
     ("tile256", 1, 256, 1), ("tile256", 300, 384, 129), ("tile256", 257, 640, 128), ("tile256", 512, 1024, 264),
