@@ -28,6 +28,7 @@ SOURCES = [
     "gated_backward.hip",
     "gated_x16.hip",
     "gated_rows.hip",
+    "gated_dots.hip",
     "dropout.hip",
     "index.hip",
     "gemm.hip",

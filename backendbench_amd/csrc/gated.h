@@ -103,9 +103,11 @@ bool gated_x16_takes(const GatedArgs& a);
 int launch_gated_x16(const GatedArgs& a, hipStream_t st);
 // gemm.hip: 128 rows by 64 features per workgroup; K % 64 == 0, 16-byte aligned rows
 int launch_gated_small2(const GatedArgs& a, hipStream_t st);
-// gated_rows.hip: at most this many rows, aligned or at any address
-constexpr int64_t kGatedRows = 64, kGatedRowsAnywhere = 4;
+// gated_rows.hip: few 16-byte aligned rows
 bool gated_rows_takes(const GatedArgs& a);
 int launch_gated_rows(const GatedArgs& a, hipStream_t st);
+// gated_dots.hip: a handful of rows of any float type, at any address
+bool gated_dots_takes(const GatedArgs& a);
+int launch_gated_dots(const GatedArgs& a, hipStream_t st);
 
 }  // namespace mi355

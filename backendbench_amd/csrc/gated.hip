@@ -88,16 +88,16 @@ extern "C" int mi355_gated_linear(const void* x, int64_t x_rs, const void* weigh
                 (long long)w_rs, (long long)K);
   const GatedArgs a{x, weight, h, pre, x_rs, w_rs, M, F, K, act, dtype};
   hipStream_t st = static_cast<hipStream_t>(stream);
+  const char* form = knobs().gated_form;  // a test and measurement knob: one form, where it applies
+  const bool dots = gated_dots_takes(a);
+  if (dots && strcmp(form, "dots") == 0) return launch_gated_dots(a, st);
   if ((dtype == MI355_BF16 || dtype == MI355_F16) && M < (1 << 30) && F < (1 << 29) && K > 0 && K < (1 << 30)) {
     const int64_t tiles = ((M + 127) / 128) * ((F + 63) / 64);  // of 128 rows by 64 features
     const bool rows16 = a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && aligned16(x) && aligned16(weight);
     const bool few = gated_rows_takes(a), t128 = rows16 && K % 64 == 0 && tiles < (1 << 23), t256 = rows16 && gated_x16_takes(a);
-    const char* form = knobs().gated_form;  // a test and measurement knob: one form, where it applies
-    if (form[0] != 0) {
-      if ((few && strcmp(form, "rows") == 0) || (M <= 16 && strcmp(form, "direct") == 0)) return launch_gated_rows(a, st);
-      if (t128 && strcmp(form, "tile128") == 0) return launch_gated_small2(a, st);
-      if (t256 && strcmp(form, "tile256") == 0) return launch_gated_x16(a, st);
-    }
+    if (few && strcmp(form, "rows") == 0) return launch_gated_rows(a, st);
+    if (t128 && strcmp(form, "tile128") == 0) return launch_gated_small2(a, st);
+    if (t256 && strcmp(form, "tile256") == 0) return launch_gated_x16(a, st);
     // Measured ([M, 4096] x 2 * 11008, [M, 2048] x 2 * 5504 and [M, 8192] x 2 * 1376, us): rows against 128-row tiles 40 / 48,
     // 16 / 19 and 16 / 47 at 32 rows, 50 / 50, 20.6 / 20 and 29 / 48 at 64; 128- against 256-row tiles 55 / 79 and 22 / 42 with
     // 172 and 86 of the former, 23 / 43 with 172, 86 / 87 and 42 / 45 with 344, 122 / 90 and 65 / 50 with 688.
@@ -106,6 +106,7 @@ extern "C" int mi355_gated_linear(const void* x, int64_t x_rs, const void* weigh
     if (t256) return launch_gated_x16(a, st);
     if (t128 && K % 128 == 0) return launch_gated_small2(a, st);  // (K % 128 == 64 with many tiles: padded rows are faster)
   }
+  if (dots) return launch_gated_dots(a, st);
   return set_error(MI355_ERR_UNSUPPORTED, "mi355_gated_linear: no single kernel for M=%lld F=%lld K=%lld %s", (long long)M, (long long)F,
                    (long long)K, dtype_name(dtype));
 }

@@ -1,14 +1,10 @@
-// The gated projection for few rows (decoding: 1 .. 64 tokens), bf16 / f16: the weight is read once and its stream is the
-// bound (4 F K bytes); v_mfma_f32_16x16x32 with the weight rows as the first operand, the waves of a workgroup share K and
-// add their accumulators in LDS at the end.  Two forms: through LDS for aligned rows, straight into registers for the rest.
-#include <string.h>
-
+// The gated projection for few aligned rows (decoding: 1 .. 64 tokens), bf16 / f16: the weight is read once and its stream
+// is the bound (4 F K bytes); v_mfma_f32_16x16x32 with the weight rows as the first operand, the waves of a workgroup share K
+// and add their accumulators in LDS at the end.
 #include "gated.h"
 #include "gemm_shared.h"
 
 namespace mi355 {
-
-typedef uint32_t gr_any __attribute__((ext_vector_type(4), aligned(2)));  // 8 elements at any element's address
 
 // Behind the last matrix instruction on `v`, in front of its first other reader: 16 wait states, more than the 16x16x32
 // instruction needs.  Not left to the compiler: in the LDS kernel's branch for K under a chunk it put none between the last
@@ -52,7 +48,7 @@ template <typename T> __device__ __forceinline__ void store_rows(const GatedArgs
     }
 }
 
-// Aligned rows: weight and x go through LDS.  An MFMA fragment takes 64 bytes of each of 16 rows per load instruction; the
+// Weight and x go through LDS.  An MFMA fragment takes 64 bytes of each of 16 rows per load instruction; the
 // memory system delivers such requests at 4.6 - 5.0 TB/s whatever their order, and 1 KB pieces of one row at 6.4 (a [22016,
 // 4096] weight read by nothing but loads: 36 - 39 us against 28).  So both operands are requested in whole pieces straight
 // into LDS (global_load_lds, 64 units of 16 bytes), a ring of NB buffers of KC elements of each row deep, and the fragments
@@ -223,86 +219,9 @@ __global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_
   }
 }
 
-// Rows at any address, up to 16 tokens: fragments straight from global memory, eight waves to a workgroup of 16 features, gate
-// and up; the waves take turns along K, 128 elements at a time, each with its next step's loads in flight while it computes.
-// 1.8 TB/s of the weight at K = 5001 (55 us for 2 * 5001 rows and one token): the misaligned 64-byte requests are the bound.
-// A copy into aligned rows in front of the other kernel costs as much for one token and less from five on.
-constexpr int kGrSteps = 4;  // 32-k pieces of a step
-
-template <typename T>
-__global__ __launch_bounds__(64 * kRlWaves) void gated_rows_kernel(GatedArgs g) {
-  __shared__ f32x4 meet[kRlWaves][2][kWave];
-  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int lr = lane & 15, lg = lane >> 4;
-  const int64_t f0 = (int64_t)blockIdx.x * 16;
-  const int64_t f = f0 + lr < g.F ? f0 + lr : g.F - 1;  // features past the last are computed on its row and not stored
-  const T* wrow[2] = {static_cast<const T*>(g.w) + f * g.w_rs, static_cast<const T*>(g.w) + (g.F + f) * g.w_rs};
-  const T* xrow = static_cast<const T*>(g.x) + (lr < g.M ? lr : g.M - 1) * g.x_rs;
-  struct Step {
-    u32x4 w[2][kGrSteps], x[kGrSteps];
-  };
-  auto fetch = [&](int64_t k, Step& s) {
-#pragma unroll
-    for (int p = 0; p < kGrSteps; ++p) {
-      const int64_t c = k + 32 * p + 8 * lg;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) s.w[u][p] = __builtin_nontemporal_load(reinterpret_cast<const gr_any*>(wrow[u] + c));
-      s.x[p] = *reinterpret_cast<const gr_any*>(xrow + c);
-    }
-  };
-  f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
-  auto multiply = [&](const Step& s) {
-#pragma unroll
-    for (int p = 0; p < kGrSteps; ++p)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) acc[u] = GrMfma<T>::run(s.w[u][p], s.x[p], acc[u]);
-  };
-  constexpr int64_t KS = 32 * kGrSteps, ROUND = KS * kRlWaves;
-  const int64_t whole = g.K / KS * KS;  // whole steps
-  int64_t k = wave * KS;
-  if (k < whole) {
-    Step a, b;
-    fetch(k, a);
-    while (true) {  // two steps per trip, the two register sets trading places
-      const int64_t kb = k + ROUND;
-      if (kb < whole) fetch(kb, b);
-      multiply(a);
-      if (kb >= whole) break;
-      k = kb + ROUND;
-      if (k < whole) fetch(k, a);
-      multiply(b);
-      if (k >= whole) break;
-    }
-  }
-  // What is left of K, 32 elements per wave: eight elements of a row at a time when they are there, else one by one, zeros
-  // behind the end (in both operands: 0 * inf).
-  for (int64_t k1 = whole + 32 * wave; k1 < g.K; k1 += 32 * kRlWaves) {
-    const int64_t c = k1 + 8 * lg;
-    const u32x4 xv = __builtin_bit_cast(u32x4, load_some(reinterpret_cast<const uint16_t*>(xrow) + c, g.K - c));
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const u32x4 wv = __builtin_bit_cast(u32x4, load_some(reinterpret_cast<const uint16_t*>(wrow[u]) + c, g.K - c));
-      acc[u] = GrMfma<T>::run(wv, xv, acc[u]);
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < 2; ++u) settle(acc[u]);
-#pragma unroll
-  for (int u = 0; u < 2; ++u) meet[wave][u][lane] = acc[u];
-  __syncthreads();
-  if (wave != 0) return;
-  f32x4 gv = meet[0][0][lane], uv = meet[0][1][lane];  // the waves' parts, in a fixed order
-#pragma unroll
-  for (int q = 1; q < kRlWaves; ++q) {
-    gv += meet[q][0][lane];
-    uv += meet[q][1][lane];
-  }
-  store_rows<T>(g, lr, f0 + 4 * lg, gv, uv);
-}
-
 // Rows on 16-byte boundaries, of whole 16-byte units, and neighbours within a request's 32-bit byte offset.
-static bool rows_aligned(const GatedArgs& a) {
-  return a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && a.K % 8 == 0 && aligned16(a.x) && aligned16(a.w) && a.x_rs < (1 << 30) && a.w_rs < (1 << 30);
+bool gated_rows_takes(const GatedArgs& a) {
+  return a.M <= 64 && a.F < (1 << 25) && a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && a.K % 8 == 0 && aligned16(a.x) && aligned16(a.w) && a.x_rs < (1 << 30) && a.w_rs < (1 << 30);
 }
 
 template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t st) {
@@ -320,24 +239,18 @@ template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t 
     hipLaunchKernelGGL(kern, dim3((unsigned)((a.F + 8 * RB - 1) / (8 * RB))), dim3(64 * kRlWaves), bytes, st, a);
     return check_launch("mi355_gated_linear");
   };
-  if (strcmp(knobs().gated_form, "direct") != 0 && rows_aligned(a)) {
-    using Half = integral_constant<int, 512>;
-    using Quarter = integral_constant<int, 256>;
-    if (a.M <= 4) return lds(Four(), One(), Half(), Four(), Four());
-    // Blocks of 8 features (x read twice as often) where those of 16 would leave half of the CUs without one: 2 * 1376 x 8192, 16
-    // and 32 tokens, 17.3 -> 12.4 and 21.0 -> 16.3 us; 2 * 2752 x 4096 11.6 and 13.2 in blocks of 16, 14.3 and 17.8 in blocks of 8.
-    const bool few = a.F <= 8 * kNumCU;
-    if (a.M <= 16 && few) return lds(integral_constant<int, 16>(), One(), Half(), integral_constant<int, 5>(), Two());
-    if (a.M <= 16) return lds(integral_constant<int, 16>(), Two(), Half(), integral_constant<int, 3>(), Two());
-    if (a.M <= 32 && few) return lds(integral_constant<int, 32>(), One(), Quarter(), integral_constant<int, 6>(), Two());
-    if (a.M <= 32) return lds(integral_constant<int, 32>(), Two(), Quarter(), integral_constant<int, 5>(), Two());
-    return lds(integral_constant<int, 64>(), Two(), Quarter(), integral_constant<int, 3>(), Two());
-  }
-  hipLaunchKernelGGL((gated_rows_kernel<T>), dim3((unsigned)((a.F + 15) / 16)), dim3(64 * kRlWaves), 0, st, a);
-  return check_launch("mi355_gated_linear");
+  using Half = integral_constant<int, 512>;
+  using Quarter = integral_constant<int, 256>;
+  if (a.M <= 4) return lds(Four(), One(), Half(), Four(), Four());
+  // Blocks of 8 features (x read twice as often) where those of 16 would leave half of the CUs without one: 2 * 1376 x 8192, 16
+  // and 32 tokens, 17.3 -> 12.4 and 21.0 -> 16.3 us; 2 * 2752 x 4096 11.6 and 13.2 in blocks of 16, 14.3 and 17.8 in blocks of 8.
+  const bool few = a.F <= 8 * kNumCU;
+  if (a.M <= 16 && few) return lds(integral_constant<int, 16>(), One(), Half(), integral_constant<int, 5>(), Two());
+  if (a.M <= 16) return lds(integral_constant<int, 16>(), Two(), Half(), integral_constant<int, 3>(), Two());
+  if (a.M <= 32 && few) return lds(integral_constant<int, 32>(), One(), Quarter(), integral_constant<int, 6>(), Two());
+  if (a.M <= 32) return lds(integral_constant<int, 32>(), Two(), Quarter(), integral_constant<int, 5>(), Two());
+  return lds(integral_constant<int, 64>(), Two(), Quarter(), integral_constant<int, 3>(), Two());
 }
-
-bool gated_rows_takes(const GatedArgs& a) { return a.F < (1 << 25) && a.M <= (rows_aligned(a) ? kGatedRows : kGatedRowsAnywhere); }
 
 int launch_gated_rows(const GatedArgs& a, hipStream_t st) {
   return a.dtype == MI355_BF16 ? run_gated_rows<bf16_t>(a, st) : run_gated_rows<f16_t>(a, st);

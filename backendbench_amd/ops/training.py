@@ -154,16 +154,7 @@ def _padded(t, columns):
     return out
 
 
-def _gated_half(x, weight, h, pre, act):
-    """bf16 / f16: one kernel, on padded copies of the operands where no kernel takes their rows as they are."""
-    M, K = x.shape
-    F = weight.shape[0] // 2
-    code = _lib.DTYPE[x.dtype]
-    if not try_launch("mi355_gated_linear", x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), h.data_ptr(), _ptr(pre), M, F,
-                      K, act, code):
-        Kp = max((K + 127) // 128 * 128, 256)
-        x, weight = _padded(x, Kp), _padded(weight, Kp)
-        launch("mi355_gated_linear", x.data_ptr(), Kp, weight.data_ptr(), Kp, h.data_ptr(), _ptr(pre), M, F, Kp, act, code)
+_ANY_TYPE_ROWS = 8  # mi355_gated_linear takes this many in fp32 and fp64 too
 
 
 @on_gpu
@@ -174,18 +165,27 @@ def _gated_linear(input, weight, act, save_pre):
     if M == 0 or F == 0 or K == 0:  # (no terms: pre = 0 and act(0) = 0)
         h = torch.zeros((*lead, F), dtype=dtype, device=device)
         return (h, torch.zeros((*lead, 2 * F), dtype=dtype, device=device)) if save_pre else h
+    code = _lib.DTYPE[dtype]
     h = new_dense((*lead, F), dtype, device)
     x = _rows_of(input) if input.dim() == 2 else dense(input).view(M, K)
     weight = _rows_of(weight)
-    if dtype in _HALF:
+    if dtype in _HALF or M <= _ANY_TYPE_ROWS:
         pre = new_dense((*lead, 2 * F), dtype, device) if save_pre else None
-        _gated_half(x, weight, h, pre, act)
+
+        def fused(attempt, x, weight, K):
+            return attempt("mi355_gated_linear", x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), h.data_ptr(), _ptr(pre),
+                           M, F, K, act, code)
+
+        if not fused(try_launch, x, weight, K):  # rows that no kernel takes: padded ones
+            Kp = max((K + 127) // 128 * 128, 256)
+            fused(launch, _padded(x, Kp), _padded(weight, Kp), Kp)
         return (h, pre) if save_pre else h
-    if dtype == torch.float32 and M * F >= 1024 and (K % 16 or x.data_ptr() % 16 or weight.data_ptr() % 16):
-        Kp = (K + 63) // 64 * 64  # rows the fp32 matrix instructions' kernel takes
+    if dtype == torch.float32 and (K % 16 or x.data_ptr() % 16 or weight.data_ptr() % 16):
+        # rows the fp32 matrix instructions' kernel takes: [16, 5001] x 2 * 5001 173 -> 126 us with the copies, [197, 1001] x 2 * 771 31 -> 26
+        Kp = (K + 63) // 64 * 64
         x, weight = _padded(x, Kp), _padded(weight, Kp)
     pre = _gemm(x, weight.t(), None, 1.0, 0.0)
-    launch("mi355_gated_act", pre.data_ptr(), h.data_ptr(), _lib.DTYPE[dtype], M, F, act)
+    launch("mi355_gated_act", pre.data_ptr(), h.data_ptr(), code, M, F, act)
     return (h, pre.view(*lead, 2 * F)) if save_pre else h
 
 

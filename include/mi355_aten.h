@@ -89,7 +89,7 @@ int mi355_init(void);
  *   "gemm_prefetch": "0" .. "256"  workgroups per part of K that only read the operands ahead of the tiles, on
  *                 CUs a launch of one workgroup per CU leaves without a tile (cut down to the CUs left over;
  *                 unset: up to 32 where 16 and more are left and the K loop is long enough)
- *   "gated_form": "rows" | "direct" | "tile128" | "tile256"  the kernel of mi355_gated_linear
+ *   "gated_form": "rows" | "dots" | "tile128" | "tile256"  the kernel of mi355_gated_linear
  *                 (mi355_train.h), where it takes the operands
  *   "x16_spin_limit": polls of the in-launch split-K's bounded wait for a partial product
  *                 before it gives up (default 2^21, about two seconds); a test sets it to 0

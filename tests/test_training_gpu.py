@@ -261,7 +261,8 @@ def gated_form():
 
 @pytest.mark.parametrize("form,M,K,F", [
     ("rows", 1, 2048, 40), ("rows", 16, 1016, 24), ("rows", 17, 2056, 23), ("rows", 64, 4104, 129), ("rows", 33, 8, 1), ("rows", 5, 5120, 8),
-    ("direct", 1, 2048, 40), ("direct", 16, 1000, 129), ("direct", 4, 77, 9), ("direct", 3, 1331, 33),
+    ("dots", 1, 2048, 40), ("dots", 4, 1000, 129), ("dots", 4, 77, 9), ("dots", 3, 1331, 33), ("dots", 2, 4103, 1), ("dots", 2, 511, 4097),
+    ("dots", 1, 513, 5000),
     ("tile128", 1, 64, 1), ("tile128", 130, 128, 70), ("tile128", 64, 192, 64), ("tile128", 300, 256, 129), ("tile128", 257, 448, 200),
     ("tile128", 128, 1024, 336),
     ("tile256", 1, 256, 1), ("tile256", 300, 384, 129), ("tile256", 257, 640, 128), ("tile256", 512, 1024, 264),
@@ -275,6 +276,20 @@ def test_gated_linear_forms(gated_form, form, M, K, F, dtype):
     gated_form(form)
     h, pre = ops.gated_linear(x, w, act, save_pre=True)
     gated_forward_check(h, pre, x, w, act, f"{form} {M}x{K}x{F} {act}")
+    assert torch.equal(ops.gated_linear(x, w, act), h)
+
+
+@pytest.mark.parametrize("M,K,F", [(1, 1, 1), (1, 4096, 300), (2, 770, 5), (3, 255, 2049), (5, 513, 64), (8, 1027, 33), (9, 100, 33)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_linear_few_rows_at_any_address(dtype, M, K, F):
+    """Operands in odd columns of wider tensors, NaN around them."""
+    g = generator(M * K + F)
+    x, w = randn(g, M, K + 3, dtype=dtype), randn(g, 2 * F + 1, K + 5, dtype=dtype, scale=K ** -0.5)
+    x[:, :1], x[:, K + 1:], w[:, :3], w[:, K + 3:], w[2 * F:] = (float("nan"),) * 5
+    x, w = x[:, 1:K + 1], w[:2 * F, 3:K + 3]
+    act = ["silu", "gelu", "gelu_tanh"][M % 3]
+    h, pre = ops.gated_linear(x, w, act, save_pre=True)
+    gated_forward_check(h, pre, x, w, act, f"{M}x{K}x{F} {act}")
     assert torch.equal(ops.gated_linear(x, w, act), h)
 
 
