@@ -212,18 +212,30 @@ __global__ __launch_bounds__(kLbTile) void lb_tile_kernel(const T* __restrict__ 
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  // The weights of columns that are not this lane's become zeros, like their dy (0 * inf).
+  auto own_weights = [&]() {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      gamma[k].clear_unless(in[k]);
+      if constexpr (TAIL) gamma[k].clear_below(skip[k]);
+    }
+  };
   if constexpr (NV <= 2) {
     Row b;
+    fetch(base + step + grp, b);
+    own_weights();
     while (base < M) {  // two rows per trip, the two register sets trading places
-      fetch(base + step + grp, b);
       one_row(base + grp, a);
       base += step;
       if (base >= M) break;
       fetch(base + step + grp, a);
       one_row(base + grp, b);
       base += step;
+      if (base >= M) break;
+      fetch(base + step + grp, b);
     }
   } else {  // no room for a second row
+    own_weights();
     while (base < M) {
       one_row(base + grp, a);
       base += step;

@@ -161,6 +161,19 @@ def test_layer_norm_backward_infinities_stay_in_their_row():
         assert torch.equal(got[i][cols_ok], clean[i][cols_ok]) and not got[i][~cols_ok].isfinite().any()
 
 
+@pytest.mark.parametrize("rows,cols", [(3, 100), (300, 520), (2, 777), (9, 5000), (2, 16384)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_layer_norm_backward_infinite_weight(dtype, rows, cols):
+    """An infinite weight in the last column gives what the formula gives: lanes behind the row's end do not multiply it by 0."""
+    dy, x, mean, rstd, w, b = ln_case(rows, cols, dtype, dtype, 31)
+    w[-1], dy[:, -1] = float("inf"), 1.0
+    dx, dw, _ = ops.native_layer_norm_backward(dy, x, [cols], mean, rstd, w, b, [True] * 3)
+    xhat, g = (x.double() - mean.double()) * rstd.double(), dy.double() * w.double()
+    want = rstd.double() * (g - g.mean(1, keepdim=True) - xhat * (g * xhat).mean(1, keepdim=True))
+    assert torch.equal(dx.isnan(), want.isnan()) and torch.equal(dx == -float("inf"), want == -float("inf"))
+    assert dw.isfinite().all()
+
+
 def test_layer_norm_backward_repeats_bit_for_bit():
     case = ln_case(4099, 1024, torch.bfloat16, torch.float32, 10)
     first = ops.native_layer_norm_backward(case[0], case[1], [1024], *case[2:], [True] * 3)
