@@ -26,6 +26,7 @@ SOURCES = [
     "layernorm_bwd.hip",
     "gated.hip",
     "gated_backward.hip",
+    "gated_backward_rows.hip",
     "gated_x16.hip",
     "gated_rows.hip",
     "gated_dots.hip",

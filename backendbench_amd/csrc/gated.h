@@ -79,6 +79,13 @@ template <typename T, int V = 16 / sizeof(T)> __device__ __forceinline__ VecN<T,
   return v;
 }
 
+// 8 or 16 bytes at such an address.
+template <int BYTES, int ALIGN> struct AnyPart { typedef uint32_t type __attribute__((ext_vector_type(BYTES / 4), aligned(ALIGN))); };
+template <typename T, int V> __device__ __forceinline__ void store_any(T* p, const VecN<T, V>& v) {
+  using Part = typename AnyPart<sizeof(T) * V, sizeof(T)>::type;
+  *reinterpret_cast<Part*>(p) = __builtin_bit_cast(Part, v);
+}
+
 // body(ACT) with an integral constant.
 template <typename Body> static int dispatch_act(int act, const char* name, Body body) {
   switch (act) {
@@ -109,5 +116,18 @@ int launch_gated_rows(const GatedArgs& a, hipStream_t st);
 // gated_dots.hip: a handful of rows of any float type, at any address
 bool gated_dots_takes(const GatedArgs& a);
 int launch_gated_dots(const GatedArgs& a, hipStream_t st);
+
+
+// Its backward pass: dh [M][F], pre [M][2F], dx [M][K] and dw [2F][K] dense, dx or dw null when not wanted.
+struct GatedBackwardArgs {
+  const void *dh, *x, *w, *pre;
+  void *dx, *dw;
+  int64_t x_rs, w_rs, M, F, K;
+  int act, dtype;
+};
+// gated_backward_rows.hip: few rows of any type, strides and alignment
+bool gated_backward_rows_takes(int64_t M, int64_t K);
+int64_t gated_backward_rows_workspace(int64_t M, int64_t F, int64_t K, int dtype);
+int launch_gated_backward_rows(const GatedBackwardArgs& a, void* workspace, hipStream_t st);
 
 }  // namespace mi355

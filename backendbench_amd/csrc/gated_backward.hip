@@ -1,4 +1,4 @@
-// The gated projection, backward: with gate = pre[:, :F], up = pre[:, F:],
+// The gated projection, backward (up to 16 rows: gated_backward_rows.hip): with gate = pre[:, :F], up = pre[:, F:],
 //   dpre = [dh up act'(gate) | dh act(gate)],   dx = dpre W,   dW = dpre^T x.
 //
 // One elementwise kernel leaves dpre and its transpose, both in the products' types and paddings, and this library's
@@ -211,6 +211,7 @@ using namespace mi355;
 
 extern "C" int64_t mi355_gated_linear_backward_workspace_bytes(int64_t M, int64_t F, int64_t K, int dtype) {
   if (M <= 0 || F <= 0 || K <= 0 || dtype_size(dtype) < 2) return 0;
+  if (gated_backward_rows_takes(M, K)) return gated_backward_rows_workspace(M, F, K, dtype);
   int64_t most = 0;
   for (int aligned = 0; aligned < 4; ++aligned)
     for (int wanted = 1; wanted < 4; ++wanted) {
@@ -233,6 +234,13 @@ extern "C" int mi355_gated_linear_backward(const void* dh, const void* x, int64_
   MI355_REQUIRE(dh != nullptr && x != nullptr && weight != nullptr && pre != nullptr, "mi355_gated_linear_backward: NULL data pointer");
   MI355_REQUIRE(x_rs >= K && w_rs >= K, "mi355_gated_linear_backward: rows overlap (strides %lld, %lld for K = %lld)", (long long)x_rs,
                 (long long)w_rs, (long long)K);
+  if (gated_backward_rows_takes(M, K)) {
+    const int64_t need = gated_backward_rows_workspace(M, F, K, dtype);
+    MI355_REQUIRE(workspace != nullptr && workspace_bytes >= need && aligned16(workspace),
+                  "mi355_gated_linear_backward: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+    return launch_gated_backward_rows(GatedBackwardArgs{dh, x, weight, pre, dx, dweight, x_rs, w_rs, M, F, K, act, dtype}, workspace,
+                                      static_cast<hipStream_t>(stream));
+  }
   const int es = dtype_size(dtype);
   const bool any = dtype == MI355_F64;
   const GatedBackwardPlan p = plan_gated_backward(M, F, K, dtype, dx != nullptr, dweight != nullptr, rows16(weight, w_rs, es), rows16(x, x_rs, es));

@@ -57,7 +57,7 @@ int mi355_gated_act(const void* pre, void* h, int dtype, int64_t M, int64_t F, i
  * `dtype` (f32, f16, bf16, f64), then dx [M][K] = dpre W and dweight [2F][K] = dpre^T x, accumulated in fp32 (fp64).  dh
  * [M][F], pre [M][2F], dx and dweight are dense; x and weight have rows x_rs and w_rs apart.  dx or dweight may be NULL.
  * The workspace (16-byte aligned, contents undefined before and after; not shared by calls that may overlap in time)
- * holds dpre and the products' scratch: mi355_gated_linear_backward_workspace_bytes() always suffices. */
+ * holds dpre and the products' scratch, or partial sums of dx: mi355_gated_linear_backward_workspace_bytes() always suffices. */
 int64_t mi355_gated_linear_backward_workspace_bytes(int64_t M, int64_t F, int64_t K, int dtype);
 int mi355_gated_linear_backward(const void* dh, const void* x, int64_t x_rs, const void* weight, int64_t w_rs, const void* pre,
                                 void* dx, void* dweight, int64_t M, int64_t F, int64_t K, int act, int dtype,

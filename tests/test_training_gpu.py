@@ -306,6 +306,24 @@ def test_gated_linear_few_rows_at_any_address(dtype, M, K, F):
     assert torch.equal(ops.gated_linear(x, w, act), h)
 
 
+@pytest.mark.parametrize("M,K,F", [(1, 8, 1), (1, 2049, 9), (2, 511, 300), (7, 9, 65), (8, 768, 41), (9, 513, 7), (16, 1001, 130), (17, 100, 33)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_linear_backward_few_rows(dtype, M, K, F):
+    """Operands in odd columns of wider tensors, NaN around them; each gradient alone gives the same."""
+    g = generator(M + K + F)
+    x, w = randn(g, M, K + 3, dtype=dtype), randn(g, 2 * F + 1, K + 5, dtype=dtype, scale=K ** -0.5)
+    x[:, :1], x[:, K + 1:], w[:, :3], w[:, K + 3:], w[2 * F:] = (float("nan"),) * 5
+    x, w = x[:, 1:K + 1], w[:2 * F, 3:K + 3]
+    pre, dh = randn(g, M, 2 * F, dtype=dtype), randn(g, M, F, dtype=dtype)
+    act = ["silu", "gelu", "gelu_tanh"][M % 3]
+    got = ops.gated_linear_backward(dh, x, w, pre, act)
+    gated_backward_check(got, dh, x, w, pre, act, f"{M}x{K}x{F} {act}")
+    dx, none = ops.gated_linear_backward(dh, x, w, pre, act, (True, False))
+    assert none is None and torch.equal(dx, got[0])
+    none, dw = ops.gated_linear_backward(dh, x, w, pre, act, (False, True))
+    assert none is None and torch.equal(dw, got[1])
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
 def test_gated_linear_far_gates(act, dtype):
