@@ -79,6 +79,18 @@ template <typename T, int V = 16 / sizeof(T)> __device__ __forceinline__ VecN<T,
   return v;
 }
 
+// 16 bytes without their first `count` elements: the rest moves to the front, zeros follow.  The end of a row is read as the
+// 16 bytes that end with it, without a branch per element, and moved into place when it is needed.
+template <typename T> __device__ __forceinline__ u32x4 drop_front(u32x4 v, int count) {
+  const int bytes = count * (int)sizeof(T);
+  if (bytes & 8) v = u32x4{v[2], v[3], 0u, 0u};
+  if (bytes & 4) v = u32x4{v[1], v[2], v[3], 0u};
+  if constexpr (sizeof(T) == 2) {
+    if (bytes & 2) v = u32x4{__builtin_amdgcn_alignbit(v[1], v[0], 16), __builtin_amdgcn_alignbit(v[2], v[1], 16), __builtin_amdgcn_alignbit(v[3], v[2], 16), v[3] >> 16};
+  }
+  return bytes >= 16 ? u32x4{0u, 0u, 0u, 0u} : v;
+}
+
 // 8 or 16 bytes at such an address.
 template <int BYTES, int ALIGN> struct AnyPart { typedef uint32_t type __attribute__((ext_vector_type(BYTES / 4), aligned(ALIGN))); };
 template <typename T, int V> __device__ __forceinline__ void store_any(T* p, const VecN<T, V>& v) {
@@ -110,7 +122,8 @@ bool gated_x16_takes(const GatedArgs& a);
 int launch_gated_x16(const GatedArgs& a, hipStream_t st);
 // gemm.hip: 128 rows by 64 features per workgroup; K % 64 == 0, 16-byte aligned rows
 int launch_gated_small2(const GatedArgs& a, hipStream_t st);
-// gated_rows.hip: few 16-byte aligned rows
+// gated_rows.hip: few rows, 16-byte aligned ones of whole 16-byte units faster
+bool gated_rows_aligned(const GatedArgs& a);
 bool gated_rows_takes(const GatedArgs& a);
 int launch_gated_rows(const GatedArgs& a, hipStream_t st);
 // gated_dots.hip: a handful of rows of any float type, at any address

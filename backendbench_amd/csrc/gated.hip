@@ -101,6 +101,7 @@ extern "C" int mi355_gated_linear(const void* x, int64_t x_rs, const void* weigh
     // Measured ([M, 4096] x 2 * 11008, [M, 2048] x 2 * 5504 and [M, 8192] x 2 * 1376, us): rows against 128-row tiles 40 / 48,
     // 16 / 19 and 16 / 47 at 32 rows, 50 / 50, 20.6 / 20 and 29 / 48 at 64 (48 rows of the second outside a graph 18.5 / 17.0); 128- against 256-row tiles 55 / 79 and 22 / 42 with
     // 172 and 86 of the former, 23 / 43 with 172, 86 / 87 and 42 / 45 with 344, 122 / 90 and 65 / 50 with 688.
+    if (dots && !gated_rows_aligned(a)) return launch_gated_dots(a, st);
     if (few && (M <= 32 || !t128 || tiles < kNumCU / 4)) return launch_gated_rows(a, st);
     if (t128 && tiles <= (t256 ? kNumCU : 2 * kNumCU)) return launch_gated_small2(a, st);
     if (t256) return launch_gated_x16(a, st);

@@ -1,8 +1,9 @@
 // The gated projection for a handful of rows on the vector units: any float type, any strides and alignment.  The weight is
 // read once and its stream is the bound (2 F K elements); with so few rows no matrix instruction is needed to keep up, and
 // a wave can read 1 KB of one row at a time, at any address, where a fragment of a matrix instruction takes 64 bytes of
-// each of 16 rows.  Measured, us (TB/s of the weight): one row, 2 * 5001 x 5001 bf16 24 (4.2; 55 through copies in aligned
-// rows), 2 * 11008 x 4096 fp32 61 (5.9; 145 as a product and an activation kernel), bf16 31 (5.9; 30 through LDS).
+// each of 16 rows.  Measured, us (TB/s of the weight): one row, 2 * 5001 x 5001 bf16 22 (4.6; 55
+// through copies in aligned rows), 2 * 11008 x 4096 fp32 58 (6.2; 145 as a product and an activation kernel), bf16 31 (5.9;
+// 30 through LDS).
 #include "gated.h"
 
 namespace mi355 {
@@ -71,10 +72,25 @@ __global__ __launch_bounds__(64 * kGdWaves) void gated_dots_kernel(GatedArgs g) 
   if (k == whole && whole < g.K) {  // what is left of K, zeros behind its end in both operands (0 * inf): the wave whose turn it is
     Step s;
     const int64_t c = k + lane * V;
+    if (g.K >= V) {
+      const int64_t at = c + V <= g.K ? c : g.K - V, over = c - at;
+      const int drop = over < V ? (int)over : V;
+      auto end = [&](const T* p) __attribute__((always_inline)) { return *reinterpret_cast<const Any*>(p + at); };
+      u32x4 we[4], xe[MT];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s.w[r] = load_some(w[r] + c, g.K - c);
+      for (int r = 0; r < 4; ++r) we[r] = end(w[r]);
 #pragma unroll
-    for (int m = 0; m < MT; ++m) s.x[m] = load_some(x[m] + c, g.K - c);
+      for (int m = 0; m < MT; ++m) xe[m] = end(x[m]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s.w[r] = __builtin_bit_cast(VecN<T, V>, drop_front<T>(we[r], drop));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) s.x[m] = __builtin_bit_cast(VecN<T, V>, drop_front<T>(xe[m], drop));
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s.w[r] = load_some(w[r] + c, g.K - c);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) s.x[m] = load_some(x[m] + c, g.K - c);
+    }
     multiply(s);
   }
   // The 4 MT sums over the lanes: halves of the wave trade halves of the list until a lane holds one of them (4 MT - 1
@@ -136,16 +152,18 @@ template <typename T> static int run_gated_dots(const GatedArgs& a, hipStream_t 
   if (a.M == 1) return go(std::integral_constant<int, 1>());
   if (a.M == 2) return go(std::integral_constant<int, 2>());
   if constexpr (sizeof(T) > 2) {
-    if (a.M > 4) return go(std::integral_constant<int, 8>());
+    if (a.M <= 4) return go(std::integral_constant<int, 4>());
+    return go(std::integral_constant<int, 8>());
   }
-  return go(std::integral_constant<int, 4>());
+  return MI355_ERR_UNSUPPORTED;  // (gated_dots_takes)
 }
 
-// More rows make the vector units the bound: of 2 * 5001 x 5001 bf16 1, 2, 4 and 8 take 24, 32, 43 and 71 us against 55 in
-// padded rows, of 2 * 11008 x 4096 fp32 62, 61, 72 and 108 against 137 as a product.  Fewer than 2^32 threads.
+// More rows make the vector units the bound: of 2 * 5001 x 5001 bf16 1, 2 and 3 take 22, 28 and 38 us against 30, 39 and 32
+// on the matrix instructions, of 2 * 11008 x 4096 fp32 1, 2, 4 and 8 take 58, 57, 70 and 108 against 137 as a product.  Fewer
+// than 2^32 threads.
 bool gated_dots_takes(const GatedArgs& a) {
   const int size = dtype_size(a.dtype);
-  return size >= 2 && a.M <= (size == 2 ? 4 : 8) && a.F < (1 << 27) && a.K > 0;
+  return size >= 2 && a.M <= (size == 2 ? 2 : 8) && a.F < (1 << 27) && a.K > 0;
 }
 
 int launch_gated_dots(const GatedArgs& a, hipStream_t st) {

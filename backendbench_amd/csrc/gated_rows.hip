@@ -1,4 +1,4 @@
-// The gated projection for few aligned rows (decoding: 1 .. 64 tokens), bf16 / f16: the weight is read once and its stream
+// The gated projection for few rows (decoding: 1 .. 64 tokens), bf16 / f16: the weight is read once and its stream
 // is the bound (4 F K bytes); v_mfma_f32_16x16x32 with the weight rows as the first operand, the waves of a workgroup share K
 // and add their accumulators in LDS at the end.
 #include "gated.h"
@@ -68,7 +68,7 @@ template <bool STREAM> __device__ __forceinline__ void rl_fill(uint32_t lds_byte
 }
 template <int N> __device__ __forceinline__ void rl_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-template <typename T, int RX, int RB, int KC, int NB> struct RowsShape {
+template <int RX, int RB, int KC> struct RowsShape {
   static constexpr int MB = (RX + 15) / 16;            // token blocks
   static constexpr int ROWS = 16 * RB;                 // weight rows of a block
   static constexpr int UNITS = KC / 8;                 // 16-byte units of a row
@@ -79,12 +79,16 @@ template <typename T, int RX, int RB, int KC, int NB> struct RowsShape {
   static constexpr int P = KC / kRlWaves / 32;         // 32-k pieces of a wave per buffer
   static constexpr int BUF = (ROWS + RX) * KC * 2;
   static constexpr int MEET = kRlWaves * RB * MB * kWave * 16;
-  static constexpr int LDS = NB * BUF > MEET ? NB * BUF : MEET;
 };
 
-template <typename T, int RX, int RB, int KC, int NB, int WAVES_PER_SIMD>
+// ANY: rows at any address and any K, which the requests into LDS do not take.  The pieces come through registers, NB sets of
+// them in flight ahead, and are written to one of two buffers when their turn comes; the last chunk ends in zeros.  8, 32 and
+// 64 rows: 2 * 5001 x 5001 37, 43 and 62 us (57, 59 and 76 through copies in aligned rows), 2 * 8430 x 8126 67, 82 and 119
+// (144, 150 and 187), 2 * 4544 x 351 5.7, 6.6 and 11.7 (15.5, 17 and 16).  Chunks of 512 instead of 256 elements, two sets
+// ahead: 45 us for the first.
+template <typename T, int RX, int RB, int KC, int NB, int WAVES_PER_SIMD, bool ANY>
 __global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_kernel(GatedArgs g) {
-  using S = RowsShape<T, RX, RB, KC, NB>;
+  using S = RowsShape<RX, RB, KC>;
   constexpr int MB = S::MB, P = S::P, UNITS = S::UNITS, RPI = S::RPI;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // the ring; at the end the waves' accumulators
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -100,7 +104,7 @@ __global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_
   };
   const T* W = static_cast<const T*>(g.w);
   const T* X = static_cast<const T*>(g.x);
-  const int chunks = (int)(g.K / KC);
+  const int chunks = (int)(ANY ? (g.K + KC - 1) / KC : g.K / KC);
   // Rows are usually a power of two apart, so the memory channel of a piece is a matter of its k: workgroups that share an
   // L2 (every eighth) start at different chunks.
   const int turn = chunks > 0 ? (int)(blockIdx.x / kNumXCD % chunks) : 0;
@@ -130,8 +134,8 @@ __global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_
   for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) acc[rb][mb] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](int c) {
-    const unsigned char* buf = lds + (c % NB) * S::BUF;
+  auto multiply = [&](int slot) {
+    const unsigned char* buf = lds + slot * S::BUF;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
       const int u = wave * (4 * P) + 4 * p + lg;  // this lane's unit of a row
@@ -149,50 +153,96 @@ __global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_
       }
     }
   };
-  // NB - 1 buffers ahead.  Chunk c: its requests are back when only those of the NB - 2 chunks behind it are out; the barrier
-  // that follows says so for every wave, and that all have multiplied chunk c - 1, whose buffer is then refilled.
+  if constexpr (ANY) {
+    // Thread t has units t, t + 512, ... of a chunk's rows, the weight's and then x's.
+    constexpr int THREADS = 64 * kRlWaves, WN = S::ROWS * UNITS / THREADS, XN = (RX * UNITS + THREADS - 1) / THREADS;
+    const T* from[WN + XN];  // this thread's places in the first chunk
+    uint32_t to[WN + XN];
 #pragma unroll
-  for (int c = 0; c < NB - 1; ++c)
-    if (c < chunks) fill(c);
-  for (int c = 0; c < chunks; ++c) {
-    if (c + NB - 1 <= chunks) rl_wait<(NB - 2) * S::FILLS>();
-    else rl_wait<0>();  // (the last chunks: fewer are out)
-    __syncthreads();
-    if (c + NB - 1 < chunks) fill(c + NB - 1);
-    multiply(c);
-  }
-  // What is left of K, under a chunk: 32-k pieces, all requested before the first is used; rows end on a 16-byte unit, units
-  // behind the end are zeros in both operands (0 * inf).
-  const int64_t k0 = (int64_t)chunks * KC;
-  if (k0 < g.K) {
-    u32x4 w[P][RB], x[P][MB];
+    for (int q = 0; q < WN + XN; ++q) {
+      const int i = (q < WN ? q : q - WN) * THREADS + (int)threadIdx.x, r = i / UNITS % (q < WN ? S::ROWS : RX), u = i % UNITS;
+      from[q] = q < WN ? W + row_of(r) : X + (r < g.M ? r : g.M - 1) * g.x_rs;
+      to[q] = (uint32_t)((q < WN ? r : S::ROWS + r) * (KC * 2) + ((u ^ (r & 15)) << 4));
+    }
+    u32x4 piece[NB][WN + XN];
+    const int unit = (int)threadIdx.x % UNITS * 8;
+    auto fetch = [&](int c, u32x4 (&p)[WN + XN]) __attribute__((always_inline)) {
+      if (c >= chunks) return;
+      const int64_t k = (int64_t)c * KC + unit, at = k + 8 <= g.K ? k : g.K - 8;
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const int64_t k = k0 + 32 * (wave + kRlWaves * p) + 8 * lg;
-      const int64_t kc = k < g.K ? k : 0;
+      for (int q = 0; q < WN + XN; ++q) {
+        const auto* a = reinterpret_cast<const typename AnyVec<2>::type*>(from[q] + at);
+        p[q] = q < WN ? __builtin_nontemporal_load(a) : *a;
+      }
+    };
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb) w[p][rb] = *reinterpret_cast<const u32x4*>(W + row_of(rb * 16 + lr) + kc);
+    for (int c = 0; c < NB; ++c) fetch(c, piece[c]);
+    for (int c0 = 0; c0 < chunks; c0 += NB) {
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        const int64_t m = mb * 16 + lr;
-        x[p][mb] = *reinterpret_cast<const u32x4*>(X + (m < g.M ? m : g.M - 1) * g.x_rs + kc);
+      for (int n = 0; n < NB; ++n) {
+        const int c = c0 + n;
+        if (c >= chunks) break;
+        unsigned char* buf = lds + (c & 1) * S::BUF;
+#pragma unroll
+        for (int q = 0; q < WN + XN; ++q) {
+          if (c + 1 == chunks) {  // past the row's end: zeros, in both operands (0 * inf)
+            const int64_t over = (int64_t)c * KC + unit + 8 - g.K;
+            piece[n][q] = drop_front<T>(piece[n][q], over <= 0 ? 0 : over < 8 ? (int)over : 8);
+          }
+          *reinterpret_cast<u32x4*>(buf + to[q]) = piece[n][q];
+        }
+        // The barrier: chunk c is there for every wave, and every wave has multiplied chunk c - 1, whose buffer is next.
+        __syncthreads();
+        fetch(c + NB, piece[n]);
+        multiply(c & 1);
       }
     }
-    __builtin_amdgcn_sched_barrier(0);
+  } else {
+    // NB - 1 buffers ahead.  Chunk c: its requests are back when only those of the NB - 2 chunks behind it are out; the barrier
+    // that follows says so for every wave, and that all have multiplied chunk c - 1, whose buffer is then refilled.
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-      const bool in = k0 + 32 * (wave + kRlWaves * p) + 8 * lg < g.K;
+    for (int c = 0; c < NB - 1; ++c)
+      if (c < chunks) fill(c);
+    for (int c = 0; c < chunks; ++c) {
+      if (c + NB - 1 <= chunks) rl_wait<(NB - 2) * S::FILLS>();
+      else rl_wait<0>();  // (the last chunks: fewer are out)
+      __syncthreads();
+      if (c + NB - 1 < chunks) fill(c + NB - 1);
+      multiply(c % NB);
+    }
+    // What is left of K, under a chunk: 32-k pieces, all requested before the first is used; rows end on a 16-byte unit, units
+    // behind the end are zeros in both operands (0 * inf).
+    const int64_t k0 = (int64_t)chunks * KC;
+    if (k0 < g.K) {
+      u32x4 w[P][RB], x[P][MB];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int p = 0; p < P; ++p) {
+        const int64_t k = k0 + 32 * (wave + kRlWaves * p) + 8 * lg;
+        const int64_t kc = k < g.K ? k : 0;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) w[p][rb][e] = in ? w[p][rb][e] : 0u;
+        for (int rb = 0; rb < RB; ++rb) w[p][rb] = *reinterpret_cast<const u32x4*>(W + row_of(rb * 16 + lr) + kc);
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) x[p][mb][e] = in ? x[p][mb][e] : 0u;
+        for (int mb = 0; mb < MB; ++mb) {
+          const int64_t m = mb * 16 + lr;
+          x[p][mb] = *reinterpret_cast<const u32x4*>(X + (m < g.M ? m : g.M - 1) * g.x_rs + kc);
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
+      for (int p = 0; p < P; ++p) {
+        const bool in = k0 + 32 * (wave + kRlWaves * p) + 8 * lg < g.K;
 #pragma unroll
-        for (int mb = 0; mb < MB; ++mb) acc[rb][mb] = GrMfma<T>::run(w[p][rb], x[p][mb], acc[rb][mb]);
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) w[p][rb][e] = in ? w[p][rb][e] : 0u;
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) x[p][mb][e] = in ? x[p][mb][e] : 0u;
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) acc[rb][mb] = GrMfma<T>::run(w[p][rb], x[p][mb], acc[rb][mb]);
+      }
     }
   }
   // The waves' parts meet in LDS and are added in a fixed order.
@@ -220,8 +270,8 @@ __global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_
 }
 
 // Rows on 16-byte boundaries, of whole 16-byte units, and neighbours within a request's 32-bit byte offset.
-bool gated_rows_takes(const GatedArgs& a) {
-  return a.M <= 64 && a.F < (1 << 25) && a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && a.K % 8 == 0 && aligned16(a.x) && aligned16(a.w) && a.x_rs < (1 << 30) && a.w_rs < (1 << 30);
+bool gated_rows_aligned(const GatedArgs& a) {
+  return a.x_rs % 8 == 0 && a.w_rs % 8 == 0 && a.K % 8 == 0 && aligned16(a.x) && aligned16(a.w) && a.x_rs < (1 << 30) && a.w_rs < (1 << 30);
 }
 
 template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t st) {
@@ -229,10 +279,12 @@ template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t 
   using One = integral_constant<int, 1>;
   using Two = integral_constant<int, 2>;
   using Four = integral_constant<int, 4>;
-  auto lds = [&](auto rx, auto rb, auto kc, auto nb, auto waves) {
+  auto lds = [&](auto rx, auto rb, auto kc, auto nb, auto waves, auto any) {
     constexpr int RX = decltype(rx)::value, RB = decltype(rb)::value, KC = decltype(kc)::value, NB = decltype(nb)::value;
-    const auto kern = gated_rows_lds_kernel<T, RX, RB, KC, NB, decltype(waves)::value>;
-    constexpr int bytes = RowsShape<T, RX, RB, KC, NB>::LDS;
+    constexpr bool ANY = decltype(any)::value;
+    using S = RowsShape<RX, RB, KC>;
+    const auto kern = gated_rows_lds_kernel<T, RX, RB, KC, NB, decltype(waves)::value, ANY>;
+    constexpr int ring = (ANY ? 2 : NB) * S::BUF, bytes = ring > S::MEET ? ring : S::MEET;
     static std::atomic<uint64_t> devices{0};
     const int rc = allow_lds(reinterpret_cast<const void*>(kern), bytes, devices, "mi355_gated_linear");
     if (rc != MI355_OK) return rc;
@@ -241,16 +293,24 @@ template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t 
   };
   using Half = integral_constant<int, 512>;
   using Quarter = integral_constant<int, 256>;
-  if (a.M <= 4) return lds(Four(), One(), Half(), Four(), Four());
+  if (!gated_rows_aligned(a)) {
+    using Yes = std::true_type;
+    if (a.M <= 16) return lds(integral_constant<int, 16>(), Two(), Quarter(), Four(), Two(), Yes());
+    if (a.M <= 32) return lds(integral_constant<int, 32>(), Two(), Quarter(), integral_constant<int, 3>(), Two(), Yes());
+    return lds(integral_constant<int, 64>(), Two(), Quarter(), integral_constant<int, 3>(), Two(), Yes());
+  }
+  if (a.M <= 4) return lds(Four(), One(), Half(), Four(), Four(), std::false_type());
   // Blocks of 8 features (x read twice as often) where those of 16 would leave half of the CUs without one: 2 * 1376 x 8192, 16
   // and 32 tokens, 17.3 -> 12.4 and 21.0 -> 16.3 us; 2 * 2752 x 4096 11.6 and 13.2 in blocks of 16, 14.3 and 17.8 in blocks of 8.
   const bool few = a.F <= 8 * kNumCU;
-  if (a.M <= 16 && few) return lds(integral_constant<int, 16>(), One(), Half(), integral_constant<int, 5>(), Two());
-  if (a.M <= 16) return lds(integral_constant<int, 16>(), Two(), Half(), integral_constant<int, 3>(), Two());
-  if (a.M <= 32 && few) return lds(integral_constant<int, 32>(), One(), Quarter(), integral_constant<int, 6>(), Two());
-  if (a.M <= 32) return lds(integral_constant<int, 32>(), Two(), Quarter(), integral_constant<int, 5>(), Two());
-  return lds(integral_constant<int, 64>(), Two(), Quarter(), integral_constant<int, 3>(), Two());
+  if (a.M <= 16 && few) return lds(integral_constant<int, 16>(), One(), Half(), integral_constant<int, 5>(), Two(), std::false_type());
+  if (a.M <= 16) return lds(integral_constant<int, 16>(), Two(), Half(), integral_constant<int, 3>(), Two(), std::false_type());
+  if (a.M <= 32 && few) return lds(integral_constant<int, 32>(), One(), Quarter(), integral_constant<int, 6>(), Two(), std::false_type());
+  if (a.M <= 32) return lds(integral_constant<int, 32>(), Two(), Quarter(), integral_constant<int, 5>(), Two(), std::false_type());
+  return lds(integral_constant<int, 64>(), Two(), Quarter(), integral_constant<int, 3>(), Two(), std::false_type());
 }
+
+bool gated_rows_takes(const GatedArgs& a) { return a.M <= 64 && a.F < (1 << 25) && a.K >= 8; }
 
 int launch_gated_rows(const GatedArgs& a, hipStream_t st) {
   return a.dtype == MI355_BF16 ? run_gated_rows<bf16_t>(a, st) : run_gated_rows<f16_t>(a, st);

@@ -274,7 +274,7 @@ def gated_form():
 
 @pytest.mark.parametrize("form,M,K,F", [
     ("rows", 1, 2048, 40), ("rows", 16, 1016, 24), ("rows", 17, 2056, 23), ("rows", 64, 4104, 129), ("rows", 33, 8, 1), ("rows", 5, 5120, 8),
-    ("dots", 1, 2048, 40), ("dots", 4, 1000, 129), ("dots", 4, 77, 9), ("dots", 3, 1331, 33), ("dots", 2, 4103, 1), ("dots", 2, 511, 4097),
+    ("dots", 1, 2048, 40), ("dots", 2, 1000, 129), ("dots", 1, 77, 9), ("dots", 2, 1331, 33), ("dots", 2, 4103, 1), ("dots", 2, 511, 4097),
     ("dots", 1, 513, 5000),
     ("tile128", 1, 64, 1), ("tile128", 130, 128, 70), ("tile128", 64, 192, 64), ("tile128", 300, 256, 129), ("tile128", 257, 448, 200),
     ("tile128", 128, 1024, 336),
@@ -292,7 +292,8 @@ def test_gated_linear_forms(gated_form, form, M, K, F, dtype):
     assert torch.equal(ops.gated_linear(x, w, act), h)
 
 
-@pytest.mark.parametrize("M,K,F", [(1, 1, 1), (1, 4096, 300), (2, 770, 5), (3, 255, 2049), (5, 513, 64), (8, 1027, 33), (9, 100, 33)])
+@pytest.mark.parametrize("M,K,F", [(1, 1, 1), (1, 4096, 300), (2, 770, 5), (3, 255, 2049), (5, 513, 64), (8, 1027, 33), (9, 100, 33), (16, 4099, 17),
+                                   (17, 257, 40), (33, 1000, 24), (64, 777, 40), (40, 263, 9), (5, 8, 16), (64, 9, 3), (12, 7, 30)])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_gated_linear_few_rows_at_any_address(dtype, M, K, F):
     """Operands in odd columns of wider tensors, NaN around them."""
