@@ -66,19 +66,6 @@ template <int B> struct AnyVec;
 template <> struct AnyVec<2> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2))); };
 template <> struct AnyVec<4> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(4))); };
 template <> struct AnyVec<8> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(8))); };
-// The V = 16 / sizeof(T) elements from p on, of which `count` are there (the rest become zeros).
-template <typename T, int V = 16 / sizeof(T)> __device__ __forceinline__ VecN<T, V> load_some(const T* p, int64_t count) {
-  VecN<T, V> v{};
-  if (count >= V) {
-    v = __builtin_bit_cast(decltype(v), __builtin_nontemporal_load(reinterpret_cast<const typename AnyVec<sizeof(T)>::type*>(p)));
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (j < count) v.v[j] = p[j];
-  }
-  return v;
-}
-
 // 16 bytes without their first `count` elements: the rest moves to the front, zeros follow.  The end of a row is read as the
 // 16 bytes that end with it, without a branch per element, and moved into place when it is needed.
 template <typename T> __device__ __forceinline__ u32x4 drop_front(u32x4 v, int count) {
@@ -89,6 +76,23 @@ template <typename T> __device__ __forceinline__ u32x4 drop_front(u32x4 v, int c
     if (bytes & 2) v = u32x4{__builtin_amdgcn_alignbit(v[1], v[0], 16), __builtin_amdgcn_alignbit(v[2], v[1], 16), __builtin_amdgcn_alignbit(v[3], v[2], 16), v[3] >> 16};
   }
   return bytes >= 16 ? u32x4{0u, 0u, 0u, 0u} : v;
+}
+
+// The V = 16 / sizeof(T) elements of a row of n from the c-th on, zeros behind its end.  Rows of at least V: in two steps, so that
+// all loads of a thread are on their way before the first is moved; shorter rows element by element.
+template <typename T, int V = 16 / sizeof(T)> __device__ __forceinline__ u32x4 load_within(const T* row, int64_t c, int64_t n) {
+  return __builtin_nontemporal_load(reinterpret_cast<const typename AnyVec<sizeof(T)>::type*>(row + (c + V <= n ? c : n - V)));
+}
+template <typename T, int V = 16 / sizeof(T)> __device__ __forceinline__ u32x4 placed(u32x4 v, int64_t c, int64_t n) {
+  const int64_t over = c + V - n;
+  return drop_front<T>(v, over <= 0 ? 0 : over < V ? (int)over : V);
+}
+template <typename T, int V = 16 / sizeof(T)> __device__ __forceinline__ VecN<T, V> load_short(const T* row, int64_t c, int64_t n) {
+  VecN<T, V> v{};
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (c + j < n) v.v[j] = row[c + j];
+  return v;
 }
 
 // 8 or 16 bytes at such an address.

@@ -29,7 +29,8 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const B* __restrict__ src
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < items; i += (int64_t)gridDim.x * 256) {
     const int64_t r = items < (int64_t(1) << 32) ? (uint32_t)i / (uint32_t)pieces : i / pieces;
     const int64_t c = (i - r * pieces) * V;
-    st<B, V>(dst + i * V, load_some(src + r * rs + c, C - c));
+    const B* row = src + r * rs;
+    st<B, V>(dst + i * V, C < V ? load_short(row, c, C) : __builtin_bit_cast(VecN<B, V>, placed<B>(load_within(row, c, C), c, C)));
   }
 }
 

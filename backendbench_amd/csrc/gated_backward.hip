@@ -38,14 +38,35 @@ __global__ __launch_bounds__(256) void gated_dpre_kernel(const T* __restrict__ d
   __shared__ T turned[COL ? 2 : 1][COL ? kGbTile : 1][COL ? LD : 1];
   const int64_t m0 = (int64_t)(blockIdx.x / tiles_f) * TM, f0 = (int64_t)(blockIdx.x % tiles_f) * kGbTile;
   VecN<T, V> gv[PER], uv[PER], dv[PER];
+  auto column = [&](int i) { return f0 + (threadIdx.x + 256 * i) * V % kGbTile; };
+  auto row = [&](int i) {  // (tiles of 16 rows: of threads past them too; rows past M read the last, their dh becomes zero)
+    const int64_t m = m0 + (threadIdx.x + 256 * i) * V / kGbTile;
+    return m < M ? m : M - 1;
+  };
+  if (F >= V) {
+    u32x4 g[PER], u[PER], d[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = (threadIdx.x + 256 * i) * V;
-    const int64_t m = m0 + e / kGbTile, f = f0 + e % kGbTile;
-    const int64_t there = m < M && e < TM * kGbTile ? F - f : 0;
-    gv[i] = load_some(pre + m * 2 * F + f, there);
-    uv[i] = load_some(pre + m * 2 * F + F + f, there);
-    dv[i] = load_some(dh + m * F + f, there);
+    for (int i = 0; i < PER; ++i) {
+      g[i] = load_within(pre + row(i) * 2 * F, column(i), F);
+      u[i] = load_within(pre + row(i) * 2 * F + F, column(i), F);
+      d[i] = load_within(dh + row(i) * F, column(i), F);
+    }
+    const bool whole = f0 + kGbTile <= F && m0 + TM <= M;  // of the block
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int64_t c = m0 + (int64_t)(threadIdx.x + 256 * i) * V / kGbTile < M ? column(i) : F;  // (F: zeros)
+      gv[i] = __builtin_bit_cast(VecN<T, V>, whole ? g[i] : placed<T>(g[i], c, F));
+      uv[i] = __builtin_bit_cast(VecN<T, V>, whole ? u[i] : placed<T>(u[i], c, F));
+      dv[i] = __builtin_bit_cast(VecN<T, V>, whole ? d[i] : placed<T>(d[i], c, F));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int64_t c = m0 + (int64_t)(threadIdx.x + 256 * i) * V / kGbTile < M ? column(i) : F;
+      gv[i] = load_short(pre + row(i) * 2 * F, c, F);
+      uv[i] = load_short(pre + row(i) * 2 * F + F, c, F);
+      dv[i] = load_short(dh + row(i) * F, c, F);
+    }
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
@@ -103,11 +124,20 @@ __global__ __launch_bounds__(256) void turn_pad_kernel(const B* __restrict__ src
   const int64_t r0 = (int64_t)(blockIdx.x / tiles_c) * kGbTile, c0 = (int64_t)(blockIdx.x % tiles_c) * kGbTile;
   constexpr int V = 16 / sizeof(B), PER = kGbTile * kGbTile / V / 256;
   VecN<B, V> v[PER];
+  auto row = [&](int i) {  // (rows past R become zeros)
+    const int64_t r = r0 + (threadIdx.x + 256 * i) * V / kGbTile;
+    return src + (r < R ? r : R - 1) * rs;
+  };
+  auto column = [&](int i) { return r0 + (threadIdx.x + 256 * i) * V / kGbTile < R ? c0 + (threadIdx.x + 256 * i) * V % kGbTile : C; };
+  if (C >= V) {
+    u32x4 raw[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = (threadIdx.x + 256 * i) * V;
-    const int64_t r = r0 + e / kGbTile, c = c0 + e % kGbTile;
-    v[i] = load_some(src + r * rs + c, r < R ? C - c : 0);
+    for (int i = 0; i < PER; ++i) raw[i] = load_within(row(i), column(i), C);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = __builtin_bit_cast(VecN<B, V>, placed<B>(raw[i], column(i), C));
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = load_short(row(i), column(i), C);
   }
 #pragma unroll
   for (int i = 0; i < PER; ++i) {

@@ -73,23 +73,20 @@ __global__ __launch_bounds__(64 * kGdWaves) void gated_dots_kernel(GatedArgs g) 
     Step s;
     const int64_t c = k + lane * V;
     if (g.K >= V) {
-      const int64_t at = c + V <= g.K ? c : g.K - V, over = c - at;
-      const int drop = over < V ? (int)over : V;
-      auto end = [&](const T* p) __attribute__((always_inline)) { return *reinterpret_cast<const Any*>(p + at); };
       u32x4 we[4], xe[MT];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) we[r] = end(w[r]);
+      for (int r = 0; r < 4; ++r) we[r] = load_within(w[r], c, g.K);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) xe[m] = end(x[m]);
+      for (int m = 0; m < MT; ++m) xe[m] = load_within(x[m], c, g.K);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s.w[r] = __builtin_bit_cast(VecN<T, V>, drop_front<T>(we[r], drop));
+      for (int r = 0; r < 4; ++r) s.w[r] = __builtin_bit_cast(VecN<T, V>, placed<T>(we[r], c, g.K));
 #pragma unroll
-      for (int m = 0; m < MT; ++m) s.x[m] = __builtin_bit_cast(VecN<T, V>, drop_front<T>(xe[m], drop));
+      for (int m = 0; m < MT; ++m) s.x[m] = __builtin_bit_cast(VecN<T, V>, placed<T>(xe[m], c, g.K));
     } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s.w[r] = load_some(w[r] + c, g.K - c);
+      for (int r = 0; r < 4; ++r) s.w[r] = load_short(w[r], c, g.K);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) s.x[m] = load_some(x[m] + c, g.K - c);
+      for (int m = 0; m < MT; ++m) s.x[m] = load_short(x[m], c, g.K);
     }
     multiply(s);
   }

@@ -185,10 +185,7 @@ __global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_
         unsigned char* buf = lds + (c & 1) * S::BUF;
 #pragma unroll
         for (int q = 0; q < WN + XN; ++q) {
-          if (c + 1 == chunks) {  // past the row's end: zeros, in both operands (0 * inf)
-            const int64_t over = (int64_t)c * KC + unit + 8 - g.K;
-            piece[n][q] = drop_front<T>(piece[n][q], over <= 0 ? 0 : over < 8 ? (int)over : 8);
-          }
+          if (c + 1 == chunks) piece[n][q] = placed<T>(piece[n][q], (int64_t)c * KC + unit, g.K);  // zeros in both operands (0 * inf)
           *reinterpret_cast<u32x4*>(buf + to[q]) = piece[n][q];
         }
         // The barrier: chunk c is there for every wave, and every wave has multiplied chunk c - 1, whose buffer is next.
