@@ -1,5 +1,5 @@
 // The gated projection of a feed-forward block, h = act(x Wg^T) * (x Wu^T), W = [Wg; Wu] of 2F rows: which kernel takes a
-// call, and the activation as a kernel of its own behind a product (fp32, fp64, and layouts no single kernel takes).
+// call, and the activation as a kernel of its own behind a product (more than a few rows of fp32 and fp64).
 #include <string.h>
 
 #include "gated.h"
@@ -100,15 +100,17 @@ extern "C" int mi355_gated_linear(const void* x, int64_t x_rs, const void* weigh
     if (t128 && strcmp(form, "tile128") == 0) return launch_gated_small2(a, st);
     if (t256 && strcmp(form, "tile256") == 0) return launch_gated_x16(a, st);
     // Measured ([M, 4096] x 2 * 11008, [M, 2048] x 2 * 5504 and [M, 8192] x 2 * 1376, us): rows against 128-row tiles 40 / 48,
-    // 16 / 19 and 16 / 47 at 32 rows, 50 / 50, 20.6 / 20 and 29 / 48 at 64 (48 rows of the second outside a graph 18.5 / 17.0); 128- against 256-row tiles 55 / 79 and 22 / 42 with
-    // 172 and 86 of the former, 23 / 43 with 172, 86 / 87 and 42 / 45 with 344, 122 / 90 and 65 / 50 with 688.
+    // 16 / 19 and 16 / 47 at 32 rows, 50 / 50, 20.6 / 20 and 29 / 48 at 64 (48 rows of the second outside a graph 18.5 / 17.0);
+    // 128- against 256-row tiles 55 / 79 and 22 / 42 with 172 and 86 of the former, 23 / 43 with 172, 86 / 87 and 42 / 45 with
+    // 344, 122 / 90 and 65 / 50 with 688.
     if (dots && !gated_rows_aligned(a)) return launch_gated_dots(a, st);
     if (few && (M <= 32 || !t128 || tiles < kNumCU / 4)) return launch_gated_rows(a, st);
     if (t128 && tiles <= (t256 ? kNumCU : 2 * kNumCU)) return launch_gated_small2(a, st);
     if (t256) return launch_gated_x16(a, st);
     if (t128 && K % 128 == 0) return launch_gated_small2(a, st);  // (K % 128 == 64 with many tiles: padded rows are faster)
   }
-  if (dots) return launch_gated_dots(a, st);
+  if (dots && strcmp(form, "rows") != 0) return launch_gated_dots(a, st);
+  if (dtype == MI355_F32 && gated_rows_takes(a)) return launch_gated_rows(a, st);
   return set_error(MI355_ERR_UNSUPPORTED, "mi355_gated_linear: no single kernel for M=%lld F=%lld K=%lld %s", (long long)M, (long long)F,
                    (long long)K, dtype_name(dtype));
 }

@@ -150,17 +150,19 @@ template <typename T> static int run_gated_dots(const GatedArgs& a, hipStream_t 
   if (a.M == 2) return go(std::integral_constant<int, 2>());
   if constexpr (sizeof(T) > 2) {
     if (a.M <= 4) return go(std::integral_constant<int, 4>());
-    return go(std::integral_constant<int, 8>());
   }
-  return MI355_ERR_UNSUPPORTED;  // (gated_dots_takes)
+  if constexpr (sizeof(T) > 4) {
+    if (a.M <= 8) return go(std::integral_constant<int, 8>());
+  }
+  return set_error(MI355_ERR_UNSUPPORTED, "mi355_gated_linear: no vector kernel for %lld rows of %s", (long long)a.M, dtype_name(a.dtype));
 }
 
-// More rows make the vector units the bound: of 2 * 5001 x 5001 bf16 1, 2 and 3 take 22, 28 and 38 us against 30, 39 and 32
-// on the matrix instructions, of 2 * 11008 x 4096 fp32 1, 2, 4 and 8 take 58, 57, 70 and 108 against 137 as a product.  Fewer
-// than 2^32 threads.
+// More rows make the vector units the bound.  Against the matrix instructions, us: 2 * 5001 x 5001 bf16 1, 2 and 3 rows 22 / 30,
+// 28 / 39 and 38 / 32; 2 * 11008 x 4096 fp32 2, 4 and 8 rows 58 / 80, 71 / 76 and 108 / 75, 2 * 1376 x 8192 18 / 35, 21 / 33 and
+// 32 / 33.  (fp64 has no other fused form.)  Fewer than 2^32 threads.
 bool gated_dots_takes(const GatedArgs& a) {
   const int size = dtype_size(a.dtype);
-  return size >= 2 && a.M <= (size == 2 ? 2 : 8) && a.F < (1 << 27) && a.K > 0;
+  return size >= 2 && a.M <= size && a.F < (1 << 27) && a.K > 0;
 }
 
 int launch_gated_dots(const GatedArgs& a, hipStream_t st) {

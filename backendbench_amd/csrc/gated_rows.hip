@@ -1,6 +1,6 @@
-// The gated projection for few rows (decoding: 1 .. 64 tokens), bf16 / f16: the weight is read once and its stream
-// is the bound (4 F K bytes); v_mfma_f32_16x16x32 with the weight rows as the first operand, the waves of a workgroup share K
-// and add their accumulators in LDS at the end.
+// The gated projection for few rows (decoding: 1 .. 64 tokens), bf16 / f16, and up to 32 in fp32: the weight is read once and
+// its stream is the bound (2 F K elements); 16x16 matrix instructions with the weight rows as the first operand, the waves of a
+// workgroup share K and add their accumulators in LDS at the end.
 #include "gated.h"
 #include "gemm_shared.h"
 
@@ -12,7 +12,16 @@ namespace mi355 {
 // [3, 1000] x 2 * 24 f16 came out wrong).
 __device__ __forceinline__ void settle(f32x4& v) { asm volatile("s_nop 15" : "+v"(v)); }
 
+// c + a b over 64 bytes of each of 16 rows: lane (r, g) = (lane % 16, lane / 16) holds bytes 16 g .. 16 g + 15 of row r of either.
 template <typename T> struct GrMfma;
+template <> struct GrMfma<float> {  // element j of every lane: the k of 4 g + j, the same in both operands
+  static __device__ __forceinline__ f32x4 run(u32x4 a, u32x4 b, f32x4 c) {
+    const f32x4 av = __builtin_bit_cast(f32x4, a), bv = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(av[j], bv[j], c, 0, 0, 0);
+    return c;
+  }
+};
 template <> struct GrMfma<bf16_t> {
   static __device__ __forceinline__ f32x4 run(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -30,7 +39,7 @@ template <typename T> __device__ __forceinline__ void store_rows(const GatedArgs
   float hv[4];
   auto hidden = [&](auto ACT_) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) hv[e] = gv[e] * gate_q<decltype(ACT_)::value, GateHalf>(gv[e]) * uv[e];
+    for (int e = 0; e < 4; ++e) hv[e] = gv[e] * gate_q<decltype(ACT_)::value, GateMath<T>>(gv[e]) * uv[e];
   };
   if (g.act == MI355_SILU) hidden(std::integral_constant<int, MI355_SILU>{});
   else if (g.act == MI355_GELU) hidden(std::integral_constant<int, MI355_GELU>{});
@@ -68,16 +77,17 @@ template <bool STREAM> __device__ __forceinline__ void rl_fill(uint32_t lds_byte
 }
 template <int N> __device__ __forceinline__ void rl_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-template <int RX, int RB, int KC> struct RowsShape {
+// KB: bytes of a row in a buffer.
+template <int RX, int RB, int KB> struct RowsShape {
   static constexpr int MB = (RX + 15) / 16;            // token blocks
   static constexpr int ROWS = 16 * RB;                 // weight rows of a block
-  static constexpr int UNITS = KC / 8;                 // 16-byte units of a row
+  static constexpr int UNITS = KB / 16;                // 16-byte units of a row
   static constexpr int RPI = 64 / UNITS;               // rows per request
   static constexpr int WFILLS = ROWS / RPI / kRlWaves;                               // requests of a wave per buffer: weight,
   static constexpr int XFILLS = RX / RPI >= kRlWaves ? RX / RPI / kRlWaves : 1;      // x (fewer than waves: some twice)
   static constexpr int FILLS = WFILLS + XFILLS;
-  static constexpr int P = KC / kRlWaves / 32;         // 32-k pieces of a wave per buffer
-  static constexpr int BUF = (ROWS + RX) * KC * 2;
+  static constexpr int P = KB / kRlWaves / 64;         // 64-byte pieces of a wave per buffer
+  static constexpr int BUF = (ROWS + RX) * KB;
   static constexpr int MEET = kRlWaves * RB * MB * kWave * 16;
 };
 
@@ -85,10 +95,12 @@ template <int RX, int RB, int KC> struct RowsShape {
 // them in flight ahead, and are written to one of two buffers when their turn comes; the last chunk ends in zeros.  8, 32 and
 // 64 rows: 2 * 5001 x 5001 37, 43 and 62 us (57, 59 and 76 through copies in aligned rows), 2 * 8430 x 8126 67, 82 and 119
 // (144, 150 and 187), 2 * 4544 x 351 5.7, 6.6 and 11.7 (15.5, 17 and 16).  Chunks of 512 instead of 256 elements, two sets
-// ahead: 45 us for the first.
-template <typename T, int RX, int RB, int KC, int NB, int WAVES_PER_SIMD, bool ANY>
+// ahead: 45 us for the first.  fp32 (always this way): 16 and 32 rows of 2 * 11008 x 4096 76 and 94 us (a product and an
+// activation kernel 141), of 2 * 2649 x 951 9 and 11 (28), of 2 * 1376 x 8192 34 and 45 (38 and 39).
+template <typename T, int RX, int RB, int KB, int NB, int WAVES_PER_SIMD, bool ANY>
 __global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_kernel(GatedArgs g) {
-  using S = RowsShape<RX, RB, KC>;
+  using S = RowsShape<RX, RB, KB>;
+  constexpr int V = 16 / sizeof(T), KC = KB / sizeof(T);  // elements of a unit, of a row in a buffer
   constexpr int MB = S::MB, P = S::P, UNITS = S::UNITS, RPI = S::RPI;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // the ring; at the end the waves' accumulators
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -118,7 +130,7 @@ __global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_
       const int64_t row0 = row_of(first);
       uint32_t off = (uint32_t)(((lane % UNITS) ^ ((first + lane / UNITS) & 15)) * 16);
       if constexpr (RPI > 1) off += lane / UNITS ? (uint32_t)((row_of(first + 1) - row0) * 2) : 0u;  // (rows 2 i, 2 i + 1: neighbours)
-      rl_fill<true>(buf + first * (KC * 2), off, W + row0 + k);
+      rl_fill<true>(buf + first * KB, off, W + row0 + k);
     }
 #pragma unroll
     for (int q = 0; q < S::XFILLS; ++q) {
@@ -126,7 +138,7 @@ __global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_
       const int64_t m0 = first < g.M ? first : g.M - 1, m1 = first + 1 < g.M ? first + 1 : g.M - 1;
       uint32_t off = (uint32_t)(((lane % UNITS) ^ ((first + lane / UNITS) & 15)) * 16);
       if constexpr (RPI > 1) off += lane / UNITS ? (uint32_t)((m1 - m0) * g.x_rs * 2) : 0u;
-      rl_fill<false>(buf + (S::ROWS + first) * (KC * 2), off, X + m0 * g.x_rs + k);
+      rl_fill<false>(buf + (S::ROWS + first) * KB, off, X + m0 * g.x_rs + k);
     }
   };
   f32x4 acc[RB][MB];
@@ -143,11 +155,11 @@ __global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
         const int r = (mb * 16 + lr) % RX;  // (tokens past RX repeat: never stored)
-        x[mb] = *reinterpret_cast<const u32x4*>(buf + (S::ROWS + r) * (KC * 2) + ((u ^ (r & 15)) << 4));
+        x[mb] = *reinterpret_cast<const u32x4*>(buf + (S::ROWS + r) * KB + ((u ^ (r & 15)) << 4));
       }
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(buf + (rb * 16 + lr) * (KC * 2) + ((u ^ lr) << 4));
+        const u32x4 w = *reinterpret_cast<const u32x4*>(buf + (rb * 16 + lr) * KB + ((u ^ lr) << 4));
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) acc[rb][mb] = GrMfma<T>::run(w, x[mb], acc[rb][mb]);
       }
@@ -162,16 +174,16 @@ __global__ __launch_bounds__(64 * kRlWaves, WAVES_PER_SIMD) void gated_rows_lds_
     for (int q = 0; q < WN + XN; ++q) {
       const int i = (q < WN ? q : q - WN) * THREADS + (int)threadIdx.x, r = i / UNITS % (q < WN ? S::ROWS : RX), u = i % UNITS;
       from[q] = q < WN ? W + row_of(r) : X + (r < g.M ? r : g.M - 1) * g.x_rs;
-      to[q] = (uint32_t)((q < WN ? r : S::ROWS + r) * (KC * 2) + ((u ^ (r & 15)) << 4));
+      to[q] = (uint32_t)((q < WN ? r : S::ROWS + r) * KB + ((u ^ (r & 15)) << 4));
     }
     u32x4 piece[NB][WN + XN];
-    const int unit = (int)threadIdx.x % UNITS * 8;
+    const int unit = (int)threadIdx.x % UNITS * V;
     auto fetch = [&](int c, u32x4 (&p)[WN + XN]) __attribute__((always_inline)) {
       if (c >= chunks) return;
-      const int64_t k = (int64_t)c * KC + unit, at = k + 8 <= g.K ? k : g.K - 8;
+      const int64_t k = (int64_t)c * KC + unit, at = k + V <= g.K ? k : g.K - V;
 #pragma unroll
       for (int q = 0; q < WN + XN; ++q) {
-        const auto* a = reinterpret_cast<const typename AnyVec<2>::type*>(from[q] + at);
+        const auto* a = reinterpret_cast<const typename AnyVec<sizeof(T)>::type*>(from[q] + at);
         p[q] = q < WN ? __builtin_nontemporal_load(a) : *a;
       }
     };
@@ -276,11 +288,11 @@ template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t 
   using One = integral_constant<int, 1>;
   using Two = integral_constant<int, 2>;
   using Four = integral_constant<int, 4>;
-  auto lds = [&](auto rx, auto rb, auto kc, auto nb, auto waves, auto any) {
-    constexpr int RX = decltype(rx)::value, RB = decltype(rb)::value, KC = decltype(kc)::value, NB = decltype(nb)::value;
+  auto lds = [&](auto rx, auto rb, auto kb, auto nb, auto waves, auto any) {
+    constexpr int RX = decltype(rx)::value, RB = decltype(rb)::value, KB = decltype(kb)::value, NB = decltype(nb)::value;
     constexpr bool ANY = decltype(any)::value;
-    using S = RowsShape<RX, RB, KC>;
-    const auto kern = gated_rows_lds_kernel<T, RX, RB, KC, NB, decltype(waves)::value, ANY>;
+    using S = RowsShape<RX, RB, KB>;
+    const auto kern = gated_rows_lds_kernel<T, RX, RB, KB, NB, decltype(waves)::value, ANY>;
     constexpr int ring = (ANY ? 2 : NB) * S::BUF, bytes = ring > S::MEET ? ring : S::MEET;
     static std::atomic<uint64_t> devices{0};
     const int rc = allow_lds(reinterpret_cast<const void*>(kern), bytes, devices, "mi355_gated_linear");
@@ -288,28 +300,35 @@ template <typename T> static int run_gated_rows(const GatedArgs& a, hipStream_t 
     hipLaunchKernelGGL(kern, dim3((unsigned)((a.F + 8 * RB - 1) / (8 * RB))), dim3(64 * kRlWaves), bytes, st, a);
     return check_launch("mi355_gated_linear");
   };
+  using Whole = integral_constant<int, 1024>;  // a request's
   using Half = integral_constant<int, 512>;
-  using Quarter = integral_constant<int, 256>;
-  if (!gated_rows_aligned(a)) {
-    using Yes = std::true_type;
-    if (a.M <= 16) return lds(integral_constant<int, 16>(), Two(), Quarter(), Four(), Two(), Yes());
-    if (a.M <= 32) return lds(integral_constant<int, 32>(), Two(), Quarter(), integral_constant<int, 3>(), Two(), Yes());
-    return lds(integral_constant<int, 64>(), Two(), Quarter(), integral_constant<int, 3>(), Two(), Yes());
-  }
-  if (a.M <= 4) return lds(Four(), One(), Half(), Four(), Four(), std::false_type());
   // Blocks of 8 features (x read twice as often) where those of 16 would leave half of the CUs without one: 2 * 1376 x 8192, 16
   // and 32 tokens, 17.3 -> 12.4 and 21.0 -> 16.3 us; 2 * 2752 x 4096 11.6 and 13.2 in blocks of 16, 14.3 and 17.8 in blocks of 8.
   const bool few = a.F <= 8 * kNumCU;
-  if (a.M <= 16 && few) return lds(integral_constant<int, 16>(), One(), Half(), integral_constant<int, 5>(), Two(), std::false_type());
-  if (a.M <= 16) return lds(integral_constant<int, 16>(), Two(), Half(), integral_constant<int, 3>(), Two(), std::false_type());
-  if (a.M <= 32 && few) return lds(integral_constant<int, 32>(), One(), Quarter(), integral_constant<int, 6>(), Two(), std::false_type());
-  if (a.M <= 32) return lds(integral_constant<int, 32>(), Two(), Quarter(), integral_constant<int, 5>(), Two(), std::false_type());
-  return lds(integral_constant<int, 64>(), Two(), Quarter(), integral_constant<int, 3>(), Two(), std::false_type());
+  if (sizeof(T) == 4 || !gated_rows_aligned(a)) {
+    using Yes = std::true_type;
+    if (a.M <= 16 && few) return lds(integral_constant<int, 16>(), One(), Half(), integral_constant<int, 6>(), Two(), Yes());
+    if (a.M <= 16) return lds(integral_constant<int, 16>(), Two(), Half(), Four(), Two(), Yes());
+    if (a.M <= 32 && few) return lds(integral_constant<int, 32>(), One(), Half(), Four(), Two(), Yes());
+    if (a.M <= 32) return lds(integral_constant<int, 32>(), Two(), Half(), integral_constant<int, 3>(), Two(), Yes());
+    if constexpr (sizeof(T) == 2) return lds(integral_constant<int, 64>(), Two(), Half(), integral_constant<int, 3>(), Two(), Yes());
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (a.M <= 4) return lds(Four(), One(), Whole(), Four(), Four(), std::false_type());
+    if (a.M <= 16 && few) return lds(integral_constant<int, 16>(), One(), Whole(), integral_constant<int, 5>(), Two(), std::false_type());
+    if (a.M <= 16) return lds(integral_constant<int, 16>(), Two(), Whole(), integral_constant<int, 3>(), Two(), std::false_type());
+    if (a.M <= 32 && few) return lds(integral_constant<int, 32>(), One(), Half(), integral_constant<int, 6>(), Two(), std::false_type());
+    if (a.M <= 32) return lds(integral_constant<int, 32>(), Two(), Half(), integral_constant<int, 5>(), Two(), std::false_type());
+    return lds(integral_constant<int, 64>(), Two(), Half(), integral_constant<int, 3>(), Two(), std::false_type());
+  }
+  return set_error(MI355_ERR_UNSUPPORTED, "mi355_gated_linear: %lld rows are not few", (long long)a.M);
 }
 
-bool gated_rows_takes(const GatedArgs& a) { return a.M <= 64 && a.F < (1 << 25) && a.K >= 8; }
+// fp32 up to 32 rows: 33 of them take 183 us at 2 * 11008 x 4096 (142 as a product), where 32 take 94.
+bool gated_rows_takes(const GatedArgs& a) { return a.M <= (a.dtype == MI355_F32 ? 32 : 64) && a.F < (1 << 25) && a.K >= 8 && a.K < (1 << 30); }
 
 int launch_gated_rows(const GatedArgs& a, hipStream_t st) {
+  if (a.dtype == MI355_F32) return run_gated_rows<float>(a, st);
   return a.dtype == MI355_BF16 ? run_gated_rows<bf16_t>(a, st) : run_gated_rows<f16_t>(a, st);
 }
 

@@ -154,7 +154,7 @@ def _padded(t, columns):
     return out
 
 
-_ANY_TYPE_ROWS = 8  # mi355_gated_linear takes this many in fp32 and fp64 too
+_WIDE_ROWS = {torch.float32: 32, torch.float64: 8}  # mi355_gated_linear takes up to this many
 
 
 @on_gpu
@@ -169,19 +169,22 @@ def _gated_linear(input, weight, act, save_pre):
     h = new_dense((*lead, F), dtype, device)
     x = _rows_of(input) if input.dim() == 2 else dense(input).view(M, K)
     weight = _rows_of(weight)
-    if dtype in _HALF or M <= _ANY_TYPE_ROWS:
+    if dtype in _HALF or M <= _WIDE_ROWS[dtype]:
         pre = new_dense((*lead, 2 * F), dtype, device) if save_pre else None
 
         def fused(attempt, x, weight, K):
             return attempt("mi355_gated_linear", x.data_ptr(), x.stride(0), weight.data_ptr(), weight.stride(0), h.data_ptr(), _ptr(pre),
                            M, F, K, act, code)
 
-        if not fused(try_launch, x, weight, K):  # rows that no kernel takes: padded ones
+        done = fused(try_launch, x, weight, K)
+        if not done and dtype in _HALF:  # rows that no kernel takes: padded ones
             Kp = max((K + 127) // 128 * 128, 256)
             fused(launch, _padded(x, Kp), _padded(weight, Kp), Kp)
-        return (h, pre) if save_pre else h
+            done = True
+        if done:
+            return (h, pre) if save_pre else h
     if dtype == torch.float32 and (K % 16 or x.data_ptr() % 16 or weight.data_ptr() % 16):
-        # rows the fp32 matrix instructions' kernel takes: [16, 5001] x 2 * 5001 173 -> 126 us with the copies, [197, 1001] x 2 * 771 31 -> 26
+        # rows the fp32 matrix instructions' kernel takes: [64, 5001] x 2 * 5001 180 -> 131 us with the copies, [64, 1001] x 2 * 771 21 -> 17
         Kp = (K + 63) // 64 * 64
         x, weight = _padded(x, Kp), _padded(weight, Kp)
     pre = _gemm(x, weight.t(), None, 1.0, 0.0)

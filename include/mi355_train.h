@@ -39,9 +39,9 @@ typedef enum mi355_activation {
 /* h = act(x Wg^T) * (x Wu^T) in one kernel: x [M][K] with rows x_rs apart, weight [2F][K] = [Wg; Wu] with rows w_rs
  * apart, both unit-stride along K; h [M][F] dense; pre (may be NULL) receives the pre-activations [M][2F], dense.  All of
  * `dtype` (f32, f16, bf16, f64).  Products accumulate in fp32 (fp64 for f64); the activation takes the unrounded sums.
- * Any strides and alignment: up to 64 rows of f16 or bf16 with K >= 8 (2 with any K), 8 of f32 or f64.  More rows of f16
- * and bf16 with 16-byte aligned rows and K % 128 == 0, or K % 64 == 0 and at most 512 tiles of 128 rows by 64 features.
- * Otherwise MI355_ERR_UNSUPPORTED with nothing launched: mi355_pad_rows brings f16 and bf16 operands into rows that are
+ * Any strides and alignment: with K >= 8 up to 64 rows of f16 or bf16, 32 of f32; with any K 2 of f16 or bf16, 4 of f32, 8
+ * of f64.  More rows of f16 and bf16 with 16-byte aligned rows and K % 128 == 0, or K % 64 == 0 and at most 512 tiles of
+ * 128 rows by 64 features.  Otherwise MI355_ERR_UNSUPPORTED with nothing launched: mi355_pad_rows brings f16 and bf16 operands into rows that are
  * taken; more rows of f32 and f64 are a product followed by mi355_gated_act. */
 int mi355_gated_linear(const void* x, int64_t x_rs, const void* weight, int64_t w_rs, void* h, void* pre, int64_t M, int64_t F,
                        int64_t K, int act, int dtype, void* stream);

@@ -162,7 +162,7 @@ def test_c_entry_points_check_their_arguments():
     refused(fwd(p, 63, p, 64, p, None, 4, 8, 64, 0, _lib.BF16, None), b"overlap")
     refused(fwd(p, 64, p, 0, p, None, 4, 8, 64, 0, _lib.BF16, None), b"overlap")
     refused(fwd(p, 64, p, 64, p, None, 4, -8, 64, 0, _lib.BF16, None), b"negative")
-    for rows, K, dtype in ((9, 64, _lib.F32), (9, 64, _lib.F64), (4, 64, _lib.I8), (4, 64, _lib.I32), (65, 63, _lib.BF16), (65, 72, _lib.F16), (5, 7, _lib.BF16),
+    for rows, K, dtype in ((33, 64, _lib.F32), (5, 7, _lib.F32), (9, 64, _lib.F64), (4, 64, _lib.I8), (4, 64, _lib.I32), (65, 63, _lib.BF16), (65, 72, _lib.F16), (5, 7, _lib.BF16),
                            (4, 0, _lib.BF16)):
         assert fwd(p, K, p, K, p, None, rows, 8, K, 0, dtype, None) == -2     # unsupported, nothing launched
     assert fwd(None, 64, None, 64, None, None, 0, 8, 64, 0, _lib.BF16, None) == 0
