@@ -10,6 +10,7 @@ calls on tensors.
 import functools
 import ctypes
 import os
+import threading
 
 import torch
 
@@ -161,27 +162,33 @@ def new_dense(shape, dtype, device):
 # shape, dtype, device and layout are the ones it would have allocated.  The kernel then writes
 # straight into `out`: no temporary, no second pass.  Anything else (a resize, a cast, an `out`
 # that shares memory with an input) leaves the offer untaken and the overload copies as before.
-_offered = []
+# An offer is its thread's own: autograd runs gradients on worker threads while another thread may be inside an out= overload.
+class _Offered(threading.local):
+    def __init__(self):
+        self.outs = []
+
+
+_offered = _Offered()
 
 
 def offer_out(*outs):
-    _offered[:] = outs
+    _offered.outs[:] = outs
 
 
 def withdraw_out():
-    _offered.clear()
+    _offered.outs.clear()
 
 
 def _take(shape, dtype, device, strides):
-    for i, t in enumerate(_offered):
+    for i, t in enumerate(_offered.outs):
         if t.dtype == dtype and t.device == device and tuple(t.shape) == tuple(shape) and t.stride() == tuple(strides):
-            return _offered.pop(i)
+            return _offered.outs.pop(i)
     return None
 
 
 def new_result(shape, dtype, device):
     """Row-major buffer for an operator's result: the offered out= tensor when it fits, else a new one."""
-    if _offered:
+    if _offered.outs:
         t = _take(shape, dtype, device, row_major_strides(shape))
         if t is not None:
             return t
@@ -192,7 +199,7 @@ def result_like(lead, dtype):
     """Result buffer with the (permuted-dense) layout of `lead`: the offered out= tensor when it has exactly
     that layout, else torch.empty_like's."""
     out = torch.empty_like(lead) if lead.dtype == dtype else torch.empty_like(lead, dtype=dtype)
-    if _offered:
+    if _offered.outs:
         t = _take(out.shape, dtype, out.device, out.stride())
         if t is not None:
             return t
