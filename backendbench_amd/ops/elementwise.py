@@ -448,12 +448,20 @@ def _shares_memory(out, args, kwargs):
     return False
 
 
+def _meet(outs):
+    """True when two of `outs` have memory in common."""
+    spans = sorted((o.data_ptr(), o.data_ptr() + (sum((n - 1) * s for n, s in zip(o.shape, o.stride())) + 1) * o.element_size())
+                   for o in outs if o.numel())
+    return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+
+
 def _call_into(functional, outs, args, kwargs):
     """functional(*args, **kwargs) with `outs` offered as result buffers (see _common.offer_out): GPU tensors
     that share no storage with an argument - a kernel writing its result over an operand it is still
-    reading would be a race the functional form does not have."""
+    reading would be a race the functional form does not have - and no memory with each other: those are
+    stored one after the other, so that the last result stands."""
     direct = [o for o in outs if o.is_cuda and not _shares_memory(o, args, kwargs)]
-    if len(direct) != len(outs):
+    if len(direct) != len(outs) or (len(outs) > 1 and _meet(outs)):
         return functional(*args, **kwargs)
     offer_out(*direct)
     try:

@@ -5,7 +5,7 @@ import threading
 
 import torch
 
-from backendbench_amd.ops import _common
+from backendbench_amd.ops import _common, elementwise
 
 
 def on_another_thread(fn):
@@ -29,3 +29,11 @@ def test_an_offered_out_tensor_is_its_threads_own():
         assert _common.new_result((3, 4), torch.float32, cpu) is not out  # taken
     finally:
         _common.withdraw_out()
+
+
+def test_out_tensors_with_memory_in_common_are_seen():
+    base = torch.zeros(6, 8)
+    meets = elementwise._meet
+    assert meets([base, base]) and meets([base[:3], base[2:]]) and meets([base[1], torch.zeros(2), base[1, 4:]])
+    assert meets([base[:, :2], base[:, 2:]])  # interleaved: a span, not an element list
+    assert not meets([base[:3], base[3:]]) and not meets([base[0], base[5], torch.zeros(8)]) and not meets([base[:0], base])

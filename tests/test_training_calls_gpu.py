@@ -38,3 +38,15 @@ def test_layer_norm_backward_beside_an_out_overload_on_another_thread():
     ln_check(got, dy, x, mean, rstd, w, rows, cols, "beside an out= overload")
     assert len(box) == 2 and all((o == 1.0).all() for o in outs)
     assert not {t.data_ptr() for t in got} & {o.data_ptr() for o in outs}
+
+
+def test_layer_norm_backward_into_out_tensors_that_share_memory():
+    """Results that go to the same memory are stored one after the other: the last one stands, whole."""
+    rows, cols = 300, 512
+    dy, x, mean, rstd, w, b = ln_case(rows, cols, torch.float32, torch.float32, 52)
+    same, dx = torch.full_like(w, 3.0), torch.full_like(x, 3.0)
+    ops.native_layer_norm_backward_out(dy, x, [cols], mean, rstd, w, b, [True] * 3, out0=dx, out1=same, out2=same)
+    ln_check([dx, None, same], dy, x, mean, rstd, w, rows, cols, "one tensor twice")
+    part = torch.full((cols + 64,), 3.0, device="cuda")
+    ops.native_layer_norm_backward_out(dy, x, [cols], mean, rstd, w, b, [True] * 3, out0=dx, out1=part[:cols], out2=part[64:])
+    ln_check([dx, None, part[64:]], dy, x, mean, rstd, w, rows, cols, "overlapping")
