@@ -85,6 +85,7 @@ extern "C" int mi355_gated_linear(const void* x, int64_t x_rs, const void* weigh
   MI355_REQUIRE(act >= MI355_SILU && act <= MI355_GELU_TANH, "mi355_gated_linear: unknown activation %d", act);
   if (M == 0 || F == 0) return MI355_OK;
   MI355_REQUIRE(x != nullptr && weight != nullptr && h != nullptr, "mi355_gated_linear: NULL data pointer");
+  if (M == 1) x_rs = K;  // (nothing is read at that distance)
   MI355_REQUIRE(x_rs >= K && w_rs >= K, "mi355_gated_linear: rows overlap (strides %lld, %lld for K = %lld)", (long long)x_rs,
                 (long long)w_rs, (long long)K);
   const GatedArgs a{x, weight, h, pre, x_rs, w_rs, M, F, K, act, dtype};

@@ -262,6 +262,7 @@ extern "C" int mi355_gated_linear_backward(const void* dh, const void* x, int64_
   MI355_REQUIRE(M > 0 && F > 0 && K > 0, "mi355_gated_linear_backward: an empty extent: the gradients are zeros or empty, which this call does not write");
   MI355_REQUIRE(M < (1 << 30) && F < (1 << 29) && K < (1 << 30), "mi355_gated_linear_backward: extents too large");
   MI355_REQUIRE(dh != nullptr && x != nullptr && weight != nullptr && pre != nullptr, "mi355_gated_linear_backward: NULL data pointer");
+  if (M == 1) x_rs = K;  // (nothing is read at that distance)
   MI355_REQUIRE(x_rs >= K && w_rs >= K, "mi355_gated_linear_backward: rows overlap (strides %lld, %lld for K = %lld)", (long long)x_rs,
                 (long long)w_rs, (long long)K);
   if (gated_backward_rows_takes(M, K)) {

@@ -143,7 +143,10 @@ def gated_linear(input, weight, activation="silu", save_pre=False):
 
 
 def _rows_of(t):
-    """`t` [R, K] itself when its rows are unit-stride and do not overlap, else a dense copy."""
+    """`t` [R, K] itself when its rows are unit-stride and do not overlap, else a dense copy; one row K apart from the next
+    (a tensor's own stride along a dimension of 1 says nothing: a column's transpose has 1)."""
+    if t.shape[0] == 1:
+        return dense(t).as_strided((1, t.shape[1]), (t.shape[1], 1))
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else dense(t)
 
 

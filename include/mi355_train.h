@@ -36,8 +36,8 @@ typedef enum mi355_activation {
   MI355_GELU_TANH = 2  /* g / 2 * (1 + tanh(sqrt(2 / pi) * (g + 0.044715 g^3)))     */
 } mi355_activation;
 
-/* h = act(x Wg^T) * (x Wu^T) in one kernel: x [M][K] with rows x_rs apart, weight [2F][K] = [Wg; Wu] with rows w_rs
- * apart, both unit-stride along K; h [M][F] dense; pre (may be NULL) receives the pre-activations [M][2F], dense.  All of
+/* h = act(x Wg^T) * (x Wu^T) in one kernel: x [M][K] with rows x_rs apart (one row: any x_rs), weight [2F][K] = [Wg; Wu] with
+ * rows w_rs apart, both unit-stride along K; h [M][F] dense; pre (may be NULL) receives the pre-activations [M][2F], dense.  All of
  * `dtype` (f32, f16, bf16, f64).  Products accumulate in fp32 (fp64 for f64); the activation takes the unrounded sums.
  * Any strides and alignment: with K >= 8 up to 64 rows of f16 or bf16, 32 of f32; with any K 2 of f16 or bf16, 4 of f32, 8
  * of f64.  More rows of f16 and bf16 with 16-byte aligned rows and K % 128 == 0, or K % 64 == 0 and at most 512 tiles of
@@ -55,7 +55,7 @@ int mi355_gated_act(const void* pre, void* h, int dtype, int64_t M, int64_t F, i
 
 /* The gated projection's gradients: dpre = [dh * up * act'(gate) | dh * act(gate)] with gate = pre[m][f], up = pre[m][F + f], rounded once to
  * `dtype` (f32, f16, bf16, f64), then dx [M][K] = dpre W and dweight [2F][K] = dpre^T x, accumulated in fp32 (fp64).  dh
- * [M][F], pre [M][2F], dx and dweight are dense; x and weight have rows x_rs and w_rs apart.  dx or dweight may be NULL.
+ * [M][F], pre [M][2F], dx and dweight are dense; x and weight have rows x_rs and w_rs apart (one row of x: any x_rs).  dx or dweight may be NULL.
  * The workspace (16-byte aligned, contents undefined before and after; not shared by calls that may overlap in time)
  * holds dpre and the products' scratch, or partial sums of dx: mi355_gated_linear_backward_workspace_bytes() always suffices. */
 int64_t mi355_gated_linear_backward_workspace_bytes(int64_t M, int64_t F, int64_t K, int dtype);

@@ -8,7 +8,7 @@ import torch
 
 from backendbench_amd import ops
 from backendbench_amd.ops import elementwise
-from test_training_gpu import generator, ln_case, ln_check, randn
+from test_training_gpu import DTYPES, gated_backward_check, gated_forward_check, generator, ln_case, ln_check, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,28 @@ def test_layer_norm_backward_into_out_tensors_that_share_memory():
     part = torch.full((cols + 64,), 3.0, device="cuda")
     ops.native_layer_norm_backward_out(dy, x, [cols], mean, rstd, w, b, [True] * 3, out0=dx, out1=part[:cols], out2=part[64:])
     ln_check([dx, None, part[64:]], dy, x, mean, rstd, w, rows, cols, "overlapping")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K,F", [(1, 9), (16, 40), (17, 33), (2048, 24)])
+def test_gated_linear_one_row_of_any_stride(K, F, dtype):
+    """One token whose row stride torch reports as 1, 0 or an odd distance: the result of the dense row."""
+    g = generator(K + F)
+    w = randn(g, 2 * F, K, dtype=dtype, scale=K ** -0.5)
+    column = randn(g, K, 1, dtype=dtype)
+    dense = column.t().clone(memory_format=torch.contiguous_format).view(1, K)
+    h, pre = ops.gated_linear(dense, w, "gelu", save_pre=True)
+    gated_forward_check(h, pre, dense, w, "gelu", "dense")
+    dh = randn(g, 1, F, dtype=dtype)
+    grads = ops.gated_linear_backward(dh, dense, w, pre, "gelu")
+    gated_backward_check(grads, dh, dense, w, pre, "gelu", "dense")
+    far = torch.full((3, K + 5), float("nan"), device="cuda", dtype=dtype)[1:2, :K]
+    far.copy_(dense)
+    got, gpre = ops.gated_linear(far, w, "gelu", save_pre=True)  # (another address, so perhaps another kernel)
+    gated_forward_check(got, gpre, dense, w, "gelu", "far")
+    gated_backward_check(ops.gated_linear_backward(dh, far, w, pre, "gelu"), dh, dense, w, pre, "gelu", "far")
+    for x in (column.t(), dense[0].expand(4, K)[:1], dense.as_strided((1, K), (0, 1)), dense.view(1, 1, K).as_strided((1, 1, K), (1, 1, 1))):
+        got, gpre = ops.gated_linear(x, w, "gelu", save_pre=True)
+        assert torch.equal(got.view(1, F), h) and torch.equal(gpre.view(1, 2 * F), pre)
+        back = ops.gated_linear_backward(dh.view_as(got), x, w, gpre, "gelu")
+        assert torch.equal(back[0].view(1, K), grads[0]) and torch.equal(back[1], grads[1])
