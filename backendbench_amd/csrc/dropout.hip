@@ -2,7 +2,7 @@
 // element index) and is never stored: the backward pass computes it again.
 //
 // Generator: Philox-4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as easy as 1, 2, 3", 2011).  One
-// counter gives 128 bits, used as eight 16-bit draws: an element is dropped when its draw is below t = round(p 2^16).
+// counter gives 128 bits, used as eight 16-bit draws: an element is dropped when its draw is below t = round(p 2^16) (halves to even).
 #include "../../include/mi355_train.h"
 #include "elementwise.h"
 
@@ -93,6 +93,6 @@ extern "C" int mi355_dropout_add(const void* x, const void* residual, int dtype,
   if (n == 0) return MI355_OK;
   MI355_REQUIRE(x != nullptr && out != nullptr, "mi355_dropout_add: NULL data pointer");
   MI355_REQUIRE(reinterpret_cast<uintptr_t>(rng) % 8 == 0, "mi355_dropout_add: rng is not 8-byte aligned");
-  const uint32_t t = (uint32_t)llround(p * 65536.0);
+  const uint32_t t = (uint32_t)nearbyint(p * 65536.0);  // halves to the even neighbour
   MI355_DISPATCH_FLOAT(dtype, "mi355_dropout_add", return run_dropout<T>(x, residual, t, rng, seed, offset, out, n, static_cast<hipStream_t>(stream)));
 }

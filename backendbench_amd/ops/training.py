@@ -256,7 +256,7 @@ def dropout_add(input, residual, p, rng):
     rng: (seed, offset), two Python integers or an int64 tensor of two.  An int64 tensor on the GPU is read by the
     kernel, so a captured graph draws anew once the program has advanced it.  Element i of input (in row-major order,
     whatever its strides) takes the i % 8-th 16 bits of Philox-4x32-10 at counter offset + i // 8 under key seed and is
-    dropped when they are below t = round(p * 65536); what is kept is scaled by 65536 / (65536 - t), which makes the
+    dropped when they are below t = round(p * 65536), halves to the even neighbour; what is kept is scaled by 65536 / (65536 - t), which makes the
     expectation exact for the p that 16 bits can hold.  Advance the offset by dropout_counters(input.numel())."""
     _check_dropout(input, p, rng)
     if residual is not None and (residual.shape != input.shape or residual.dtype != input.dtype):

@@ -65,8 +65,8 @@ int mi355_gated_linear_backward(const void* dh, const void* x, int64_t x_rs, con
 
 /* ---- dropout with a residual ------------------------------------------------------- */
 
-/* out[i] = residual[i] + (draw_i >= t ? x[i] * 65536 / (65536 - t) : 0), t = round(p * 65536), over n dense elements
- * (residual NULL: 0).  draw_i is 16 bits of Philox-4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as
+/* out[i] = residual[i] + (draw_i >= t ? x[i] * 65536 / (65536 - t) : 0), t = round(p * 65536) with halves to the even
+ * neighbour, over n dense elements (residual NULL: 0).  draw_i is 16 bits of Philox-4x32-10 (Salmon, Moraes, Dror, Shaw: "Parallel random numbers: as
  * easy as 1, 2, 3", 2011): key = the 64-bit seed, counter = offset + i / 8, bits 16 (i % 8) .. + 15 of its 128 output
  * bits.  `rng` (device memory, two int64: seed, offset) is read by the kernel when it is not NULL, so that a captured
  * graph draws anew after the caller has advanced it; otherwise seed and offset are used.  n elements use up

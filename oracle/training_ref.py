@@ -61,7 +61,7 @@ def philox4x32_10(counter, key):
 
 def dropout_keep(n, p, seed, offset):
     """bool [n] on the CPU: which elements dropout keeps."""
-    t = int(math.floor(p * 65536 + 0.5))
+    t = round(p * 65536)  # halves to even
     draws = []
     for i in range((n + 7) // 8):
         ctr = (offset + i) % 2 ** 64
@@ -72,5 +72,5 @@ def dropout_keep(n, p, seed, offset):
 
 
 def dropout_scale(p):
-    t = int(math.floor(p * 65536 + 0.5))
+    t = round(p * 65536)  # halves to even
     return 65536.0 / (65536 - t) if t < 65536 else 0.0

@@ -8,6 +8,7 @@ import torch
 
 from backendbench_amd import _lib
 from backendbench_amd.ops import _common, elementwise, training
+from oracle import training_ref as ref
 
 
 def on_another_thread(fn):
@@ -67,3 +68,13 @@ def test_c_entry_points_take_one_row_of_any_stride():
         for rows, text in ((1, b"workspace"), (2, b"overlap")):
             assert lib.mi355_gated_linear_backward(p, p, stride, p, 64, p, p, p, rows, 8, 64, 0, _lib.F32, p, 0, None) == -1
             assert text in lib.mi355_last_error()
+
+
+@pytest.mark.parametrize("halves,t", [(1, 0), (3, 2), (5, 2), (7, 4), (131071, 65536)])
+def test_dropout_probabilities_halfway_between_two_steps(halves, t):
+    """p in the middle of two 65536ths goes to the even one, as the definition's round() does."""
+    p = halves * 2.0 ** -17
+    assert ref.dropout_scale(p) == (65536.0 / (65536 - t) if t < 65536 else 0.0)
+    n = 1 << 12
+    dropped = n - int(ref.dropout_keep(n, p, 3, 0).sum())
+    assert dropped == (0 if t == 0 else n) or 0 < t < 65536

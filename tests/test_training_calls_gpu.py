@@ -8,7 +8,8 @@ import torch
 
 from backendbench_amd import ops
 from backendbench_amd.ops import elementwise
-from test_training_gpu import DTYPES, gated_backward_check, gated_forward_check, generator, ln_case, ln_check, randn
+from oracle import training_ref as ref
+from test_training_gpu import DTYPES, check, gated_backward_check, gated_forward_check, generator, ln_case, ln_check, randn, unit
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +76,17 @@ def test_gated_linear_one_row_of_any_stride(K, F, dtype):
         assert torch.equal(got.view(1, F), h) and torch.equal(gpre.view(1, 2 * F), pre)
         back = ops.gated_linear_backward(dh.view_as(got), x, w, gpre, "gelu")
         assert torch.equal(back[0].view(1, K), grads[0]) and torch.equal(back[1], grads[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("halves", [1, 3, 5, 7, 65535, 131071])
+def test_dropout_probabilities_halfway_between_two_steps(halves, dtype):
+    """p in the middle of two 65536ths goes to the even one; 2^-17 is no dropout at all."""
+    p, n = halves * 2.0 ** -17, 5003
+    x = randn(generator(halves), n, dtype=dtype)
+    keep = ref.dropout_keep(n, p, 77, 5).cuda()
+    want = torch.where(keep, x.double() * ref.dropout_scale(p), 0.0)
+    got = ops.dropout_add(x, None, p, (77, 5))
+    check(got, want, 2 * unit(dtype) * want.abs(), f"p = {halves} / 2^17")
+    if halves == 1:
+        assert torch.equal(got, x)
