@@ -407,7 +407,8 @@ static LbPlan lb_plan(int64_t M, int64_t N) {
 }
 
 // Lanes per row and slabs per lane of the tile kernel; lanes == 0: the general path.  A slab is one 16-byte vector per lane
-// (single elements for rows shorter than that); two-byte rows take at most two, fp32 rows four.
+// (single elements for rows shorter than that); two-byte rows take at most two, fp32 rows four.  More than a wave of lanes
+// always hold two slabs: half as many lanes hold what one slab would.
 struct LbTile {
   int lanes, slabs;
 };
@@ -449,7 +450,7 @@ static int run_lb_tile(const LbTile& p, const T* dy, const T* x, const float* me
   constexpr int V = 16 / sizeof(T);
   const int64_t blocks = lb_tile_blocks(M, p);
   float* partial = (dw != nullptr || db != nullptr) && blocks > 1 ? ws : nullptr;
-  int rc = MI355_OK;
+  int rc = MI355_ERR_UNSUPPORTED;
 #define MI355_LB_TILE(GL_, NV_)                                                                                              \
   if (p.lanes == GL_ && p.slabs == NV_)                                                                                       \
     rc = N % V == 0 ? launch_lb_tile<T, Wt, V, GL_, NV_, false>(blocks, dy, x, mean, rstd, w, dx, partial, dw, db, M, N, st)  \
@@ -457,12 +458,12 @@ static int run_lb_tile(const LbTile& p, const T* dy, const T* x, const float* me
   if (N < V) {
     rc = launch_lb_tile<T, Wt, 1, 8, 1, false>(blocks, dy, x, mean, rstd, w, dx, partial, dw, db, M, N, st);
   } else {
-    MI355_LB_TILE(8, 1) MI355_LB_TILE(16, 1) MI355_LB_TILE(32, 1)
-    MI355_LB_TILE(64, 1) MI355_LB_TILE(128, 1) MI355_LB_TILE(256, 1) MI355_LB_TILE(512, 1) MI355_LB_TILE(1024, 1)
+    MI355_LB_TILE(8, 1) MI355_LB_TILE(16, 1) MI355_LB_TILE(32, 1) MI355_LB_TILE(64, 1)
     MI355_LB_TILE(64, 2) MI355_LB_TILE(128, 2) MI355_LB_TILE(256, 2) MI355_LB_TILE(512, 2) MI355_LB_TILE(1024, 2)
     if constexpr (sizeof(T) == 4) MI355_LB_TILE(1024, 4)
   }
 #undef MI355_LB_TILE
+  if (rc == MI355_ERR_UNSUPPORTED) return set_error(rc, "mi355_layer_norm_backward: no kernel form of %d lanes and %d slabs", p.lanes, p.slabs);
   if (rc != MI355_OK || partial == nullptr) return rc;
   hipLaunchKernelGGL((lb_finish_kernel<Wt, float>), dim3((unsigned)((2 * lb_ld(N) + 31) / 32)), dim3(kLbBlock), 0, st, partial, dw, db, N, (int)blocks);
   return check_launch("mi355_layer_norm_backward");
