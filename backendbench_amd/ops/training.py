@@ -186,8 +186,9 @@ def _gated_linear(input, weight, act, save_pre):
             done = True
         if done:
             return (h, pre) if save_pre else h
-    if dtype == torch.float32 and (K % 16 or x.data_ptr() % 16 or weight.data_ptr() % 16):
-        # rows the fp32 matrix instructions' kernel takes: [64, 5001] x 2 * 5001 180 -> 131 us with the copies, [64, 1001] x 2 * 771 21 -> 17
+    if dtype == torch.float32 and (K % 16 or any(t.data_ptr() % 16 or t.stride(0) % 4 for t in (x, weight))):
+        # rows the fp32 matrix instructions' kernel takes; the product alone: [64, 5001] x 2 * 5001 180 -> 131 us with the copies, [64, 1001] x 2 * 771 21 -> 17,
+        # [64, 4096] x 2 * 5504 and [512, 2048] x 2 * 2752 with rows K + 1 apart 363 -> 133 and 236 -> 131
         Kp = (K + 63) // 64 * 64
         x, weight = _padded(x, Kp), _padded(weight, Kp)
     pre = _gemm(x, weight.t(), None, 1.0, 0.0)

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from backendbench_amd import ops
-from backendbench_amd.ops import elementwise
+from backendbench_amd.ops import elementwise, training
 from oracle import training_ref as ref
 from test_training_gpu import DTYPES, check, gated_backward_check, gated_forward_check, generator, ln_case, ln_check, randn, unit
 
@@ -90,3 +90,17 @@ def test_dropout_probabilities_halfway_between_two_steps(halves, dtype):
     check(got, want, 2 * unit(dtype) * want.abs(), f"p = {halves} / 2^17")
     if halves == 1:
         assert torch.equal(got, x)
+
+
+@pytest.mark.parametrize("x_more,w_more", [(0, 1), (1, 0), (3, 2), (4, 8)])
+def test_gated_linear_f32_rows_off_16_bytes_go_through_padded_copies(monkeypatch, x_more, w_more):
+    """fp32, more rows than the fused kernels take: rows that do not start on 16-byte boundaries are padded like an odd K."""
+    M, K, F = 70, 256, 72
+    g = generator(61)
+    x, w = randn(g, M, K + x_more), randn(g, 2 * F, K + w_more, scale=K ** -0.5)
+    x[:, K:], w[:, K:] = float("nan"), float("nan")
+    calls, padded = [], training._padded
+    monkeypatch.setattr(training, "_padded", lambda t, columns: calls.append(columns) or padded(t, columns))
+    h, pre = ops.gated_linear(x[:, :K], w[:, :K], "silu", save_pre=True)
+    gated_forward_check(h, pre, x[:, :K].contiguous(), w[:, :K].contiguous(), "silu", f"{x_more} {w_more}")
+    assert calls == ([] if x_more % 4 == 0 and w_more % 4 == 0 else [K, K])
