@@ -100,12 +100,21 @@ extern "C" int mi355_gated_linear(const void* x, int64_t x_rs, const void* weigh
     if (few && strcmp(form, "rows") == 0) return launch_gated_rows(a, st);
     if (t128 && strcmp(form, "tile128") == 0) return launch_gated_small2(a, st);
     if (t256 && strcmp(form, "tile256") == 0) return launch_gated_x16(a, st);
-    // Measured ([M, 4096] x 2 * 11008, [M, 2048] x 2 * 5504 and [M, 8192] x 2 * 1376, us): rows against 128-row tiles 40 / 48,
-    // 16 / 19 and 16 / 47 at 32 rows, 50 / 50, 20.6 / 20 and 29 / 48 at 64 (48 rows of the second outside a graph 18.5 / 17.0);
+    // Measured, us (graphs, inputs that no cache holds).  Rows against 128-row tiles up to 32 rows: 40 / 48, 16 / 19 and 16 / 47 at
+    // [32, 4096] x 2 * 11008, [32, 2048] x 2 * 5504 and [32, 8192] x 2 * 1376.  Beyond, the rows' kernel takes one round of the CUs
+    // per 4096 features and the tiles a time that grows with K, however few they are.  64 rows (33: the rows' side 3 - 14 % less):
+    //      F   K = 512      1024         2048         2560         4096         8192
+    //   4096   6.2 /  7.8    8.3 / 10.5  13.3 / 19.6  15.9 / 28.0  21.5 / 33.8  36.3 / 65.6
+    //   4160  10.2 /  7.9   13.3 / 10.5  19.3 / 19.8  23.9 / 27.2  32.5 / 34.3  55.7 / 66.8
+    //   5504  10.5 /  7.9   13.7 / 12.2  20.8 / 20.7  25.4 / 29.0  33.2 / 36.7  61.9 / 70.1
+    //   8192  10.9 /  8.2   15.3 / 16.6  24.5 / 26.3  28.9 / 31.7  39.1 / 45.1  68.0 / 83.7
+    //   8256  14.8 /  8.2   19.7 / 16.8  29.8 / 26.5  37.2 / 31.2  50.5 / 45.8  88.7 / 88.2
+    //  11008  15.6 /  9.2   20.9 / 19.6  32.4 / 30.9  39.9 / 35.4  51.4 / 52.1  98.2 / 97.8
     // 128- against 256-row tiles 55 / 79 and 22 / 42 with 172 and 86 of the former, 23 / 43 with 172, 86 / 87 and 42 / 45 with
     // 344, 122 / 90 and 65 / 50 with 688.
+    const bool rows_win = M <= 32 || tiles <= kNumCU / 4 || (tiles <= kNumCU / 2 && K > 2048);
     if (dots && !gated_rows_aligned(a)) return launch_gated_dots(a, st);
-    if (few && (M <= 32 || !t128 || tiles < kNumCU / 4)) return launch_gated_rows(a, st);
+    if (few && (rows_win || !t128)) return launch_gated_rows(a, st);
     if (t128 && tiles <= (t256 ? kNumCU : 2 * kNumCU)) return launch_gated_small2(a, st);
     if (t256) return launch_gated_x16(a, st);
     if (t128 && K % 128 == 0) return launch_gated_small2(a, st);  // (K % 128 == 64 with many tiles: padded rows are faster)

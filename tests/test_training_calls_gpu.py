@@ -104,3 +104,13 @@ def test_gated_linear_f32_rows_off_16_bytes_go_through_padded_copies(monkeypatch
     h, pre = ops.gated_linear(x[:, :K], w[:, :K], "silu", save_pre=True)
     gated_forward_check(h, pre, x[:, :K].contiguous(), w[:, :K].contiguous(), "silu", f"{x_more} {w_more}")
     assert calls == ([] if x_more % 4 == 0 and w_more % 4 == 0 else [K, K])
+
+
+@pytest.mark.parametrize("M,K,F", [(33, 512, 4096), (64, 512, 4160), (64, 2176, 4160), (33, 2176, 8192), (40, 2048, 4104), (64, 2112, 8256)])
+def test_gated_linear_on_both_sides_of_the_rule_for_33_to_64_rows(M, K, F):
+    """One round of the CUs for the rows' kernel, two, and more; short and long K."""
+    g = generator(M + K + F)
+    x, w = randn(g, M, K, dtype=torch.bfloat16), randn(g, 2 * F, K, dtype=torch.bfloat16, scale=K ** -0.5)
+    h, pre = ops.gated_linear(x, w, "silu", save_pre=True)
+    gated_forward_check(h, pre, x, w, "silu", f"{M}x{K}x{F}")
+    assert torch.equal(ops.gated_linear(x, w, "silu"), h)
