@@ -6,10 +6,10 @@ import threading
 import pytest
 import torch
 
-from backendbench_amd import ops
+from backendbench_amd import _lib, ops
 from backendbench_amd.ops import elementwise, training
 from oracle import training_ref as ref
-from test_training_gpu import DTYPES, check, gated_backward_check, gated_forward_check, generator, ln_case, ln_check, randn, unit
+from test_training_gpu import DTYPES, HALF, check, gated_backward_check, gated_forward_check, generator, ln_case, ln_check, randn, unit
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +114,108 @@ def test_gated_linear_on_both_sides_of_the_rule_for_33_to_64_rows(M, K, F):
     h, pre = ops.gated_linear(x, w, "silu", save_pre=True)
     gated_forward_check(h, pre, x, w, "silu", f"{M}x{K}x{F}")
     assert torch.equal(ops.gated_linear(x, w, "silu"), h)
+
+
+def inside(t, before, after, rows=1):
+    """`t` [R, C] as a view of a wider, taller tensor of NaN."""
+    wide = torch.full((t.shape[0] + rows, t.shape[1] + before + after), float("nan"), device="cuda", dtype=t.dtype)
+    view = wide[:t.shape[0], before:before + t.shape[1]]
+    view.copy_(t)
+    return view
+
+
+# Many features (blocks of 16 of them), aligned rows with whole chunks and a rest behind them, and odd ones; every count of rows
+# that picks another ring.
+@pytest.mark.parametrize("M", [3, 5, 16, 17, 32, 33, 64])
+@pytest.mark.parametrize("K,F", [(1016, 2056), (4104, 2056), (264, 4099), (777, 4099), (4099, 2056)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_gated_linear_few_rows_many_features(dtype, K, F, M):
+    g = generator(M + K + F)
+    x, w = randn(g, M, K, dtype=dtype), randn(g, 2 * F, K, dtype=dtype, scale=K ** -0.5)
+    around = (8, 16) if K % 8 == 0 else (3, 2)
+    act = ["silu", "gelu", "gelu_tanh"][M % 3]
+    h, pre = ops.gated_linear(inside(x, *around), inside(w, *around), act, save_pre=True)
+    gated_forward_check(h, pre, x, w, act, f"{M}x{K}x{F} {act}")
+    assert torch.equal(ops.gated_linear(inside(x, *around), inside(w, *around), act), h)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,F", [(4, 4096, 4099), (8, 4100, 2051), (16, 2049, 4099), (12, 1032, 4200), (3, 8200, 1100)])
+def test_gated_linear_backward_few_rows_several_steps(dtype, M, K, F):
+    """A group of features takes several steps, over which the sums of dx are carried; each gradient alone gives the same."""
+    g = generator(M + K + F)
+    x, w = randn(g, M, K, dtype=dtype), randn(g, 2 * F, K, dtype=dtype, scale=K ** -0.5)
+    pre, dh = randn(g, M, 2 * F, dtype=dtype), randn(g, M, F, dtype=dtype)
+    act = ["silu", "gelu", "gelu_tanh"][F % 3]
+    xv, wv = inside(x, 1, 4), inside(w, 3, 2)
+    got = ops.gated_linear_backward(dh, xv, wv, pre, act)
+    gated_backward_check(got, dh, x, w, pre, act, f"{M}x{K}x{F} {act}")
+    dx, none = ops.gated_linear_backward(dh, xv, wv, pre, act, (True, False))
+    assert none is None and torch.equal(dx, got[0])
+    none, dw = ops.gated_linear_backward(dh, xv, wv, pre, act, (False, True))
+    assert none is None and torch.equal(dw, got[1])
+
+
+@pytest.mark.parametrize("rows,cols", [(300, 16384), (261, 16381), (600, 8200), (1030, 8193), (259, 12003)])
+@pytest.mark.parametrize("dtype,wdtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                          (torch.float16, torch.float16), (torch.float16, torch.float32)])
+def test_layer_norm_backward_long_rows_on_many_blocks(dtype, wdtype, rows, cols):
+    """Rows of 8 K - 16 K elements, a row per block at a time: several blocks with several rows each, their partial sums
+    and the pass that adds those."""
+    case = ln_case(rows, cols, dtype, wdtype, rows + cols)
+    got = ops.native_layer_norm_backward(case[0], case[1], [cols], *case[2:], [True] * 3)
+    ln_check(got, *case[:5], rows, cols, f"[{rows}, {cols}]")
+    none, dw, db = ops.native_layer_norm_backward(case[0], case[1], [cols], *case[2:], [False, True, True])
+    assert none is None and torch.equal(dw, got[1]) and torch.equal(db, got[2])
+
+
+@pytest.fixture
+def gated_form():
+    yield lambda value: _lib.set_knob("gated_form", value)
+    _lib.set_knob("gated_form", None)
+
+
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("form,M,K,F", [
+    ("dots", 2, 1331, 33), ("rows", 3, 1016, 24), ("rows", 16, 777, 2061), ("rows", 33, 520, 70), ("rows", 64, 512, 64),
+    ("tile128", 1, 64, 1), ("tile128", 130, 192, 70), ("tile128", 257, 448, 200), ("tile128", 128, 1024, 64),
+    ("tile256", 1, 256, 1), ("tile256", 300, 384, 129), ("tile256", 257, 640, 136), ("tile256", 512, 256, 256)])
+@pytest.mark.parametrize("dtype", HALF)
+def test_gated_linear_reads_and_writes_its_operands_alone(gated_form, form, M, K, F, off, dtype):
+    """Every kernel form with NaN around x and the weight and marks around h and pre, the results on and off a 16-byte boundary."""
+    g = generator(M + K + F)
+    x, w = randn(g, M, K, dtype=dtype), randn(g, 2 * F, K, dtype=dtype, scale=K ** -0.5)
+    around = (3, 2) if K % 8 else (8, 16)
+    xv, wv = inside(x, *around), inside(w, *around)
+    mark, edge = 7.0, 4096
+    out = [torch.full((edge + off + M * n + edge,), mark, device="cuda", dtype=dtype) for n in (F, 2 * F)]
+    h, pre = (o[edge + off:edge + off + M * n] for o, n in zip(out, (F, 2 * F)))
+    gated_form(form)
+    rc = _lib.load().mi355_gated_linear(xv.data_ptr(), xv.stride(0), wv.data_ptr(), wv.stride(0), h.data_ptr(), pre.data_ptr(), M, F, K,
+                                        _lib.GELU, _lib.DTYPE[dtype], _lib.current_stream_handle())
+    assert rc == 0
+    gated_forward_check(h.view(M, F), pre.view(M, 2 * F), x, w, "gelu", f"{form} {M}x{K}x{F}")
+    for o, r in zip(out, (h, pre)):
+        assert (o[:edge + off] == mark).all() and (o[edge + off + r.numel():] == mark).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,F", [(1, 8, 3), (5, 77, 33), (16, 1032, 200), (17, 40, 33), (64, 256, 64), (130, 77, 50), (257, 640, 136)])
+def test_gated_linear_backward_reads_and_writes_its_operands_alone(M, K, F, dtype):
+    """NaN around x and the weight, marks around dx, dweight and the workspace, which holds NaN before the call."""
+    g = generator(M + K + F)
+    x, w = randn(g, M, K, dtype=dtype), randn(g, 2 * F, K, dtype=dtype, scale=K ** -0.5)
+    pre, dh = randn(g, M, 2 * F, dtype=dtype), randn(g, M, F, dtype=dtype)
+    xv, wv = inside(x, 3, 2), inside(w, 8, 16)
+    lib, code, mark, edge = _lib.load(), _lib.DTYPE[dtype], 7.0, 4096
+    out = [torch.full((2 * edge + n * K,), mark, device="cuda", dtype=dtype) for n in (M, 2 * F)]
+    dx, dw = (o[edge:edge + n * K] for o, n in zip(out, (M, 2 * F)))
+    need = lib.mi355_gated_linear_backward_workspace_bytes(M, F, K, code)
+    ws = torch.full((need + 2 * edge,), 255, device="cuda", dtype=torch.uint8)
+    rc = lib.mi355_gated_linear_backward(dh.data_ptr(), xv.data_ptr(), xv.stride(0), wv.data_ptr(), wv.stride(0), pre.data_ptr(), dx.data_ptr(),
+                                         dw.data_ptr(), M, F, K, _lib.GELU, code, ws.data_ptr() + edge, need, _lib.current_stream_handle())
+    assert rc == 0
+    gated_backward_check((dx.view(M, K), dw.view(2 * F, K)), dh, x, w, pre, "gelu", f"{M}x{K}x{F}")
+    for o, r in zip(out, (dx, dw)):
+        assert (o[:edge] == mark).all() and (o[edge + r.numel():] == mark).all()
+    assert (ws[:edge] == 255).all() and (ws[edge + need:] == 255).all()
