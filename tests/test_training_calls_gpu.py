@@ -219,3 +219,62 @@ def test_gated_linear_backward_reads_and_writes_its_operands_alone(M, K, F, dtyp
     for o, r in zip(out, (dx, dw)):
         assert (o[:edge] == mark).all() and (o[edge + r.numel():] == mark).all()
     assert (ws[:edge] == 255).all() and (ws[edge + need:] == 255).all()
+
+
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("rows,cols", [(2, 5), (700, 24), (300, 136), (9, 1001), (517, 4096), (258, 9001), (5, 16500)])
+@pytest.mark.parametrize("dtype,wdtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.float16, torch.float16),
+                                          (torch.float64, torch.float64)])
+def test_layer_norm_backward_writes_its_results_alone(dtype, wdtype, rows, cols, off):
+    """Marks around the three gradients and the workspace, which holds NaN before the call; results on and off a 16-byte boundary."""
+    dy, x, mean, rstd, w, b = ln_case(rows, cols, dtype, wdtype, rows + cols)
+    lib, mark, edge = _lib.load(), 7.0, 4096
+    out = [torch.full((2 * edge + off + n,), mark, device="cuda", dtype=d) for n, d in ((rows * cols, dtype), (cols, wdtype), (cols, wdtype))]
+    got = [o[edge + off:o.numel() - edge] for o in out]
+    need = lib.mi355_layer_norm_backward_workspace_bytes(rows, cols, _lib.DTYPE[dtype])
+    ws = torch.full((need + 2 * edge,), 255, device="cuda", dtype=torch.uint8)
+    rc = lib.mi355_layer_norm_backward(dy.data_ptr(), x.data_ptr(), _lib.DTYPE[dtype], mean.data_ptr(), rstd.data_ptr(), w.data_ptr(),
+                                       _lib.DTYPE[wdtype], *(t.data_ptr() for t in got), rows, cols, ws.data_ptr() + edge, need,
+                                       _lib.current_stream_handle())
+    assert rc == 0
+    ln_check(got, dy, x, mean, rstd, w, rows, cols, f"[{rows}, {cols}]")
+    for o in out:
+        assert (o[:edge + off] == mark).all() and (o[o.numel() - edge:] == mark).all()
+    assert (ws[:edge] == 255).all() and (ws[edge + need:] == 255).all()
+
+
+def test_operators_on_two_threads_at_once():
+    """Each thread on a stream of its own, a hundred rounds of every operator: the bits of a thread alone."""
+    def work(seed):
+        g = generator(seed)
+        dt = torch.bfloat16
+        x, w = randn(g, 40, 512, dtype=dt), randn(g, 2 * 344, 512, dtype=dt, scale=0.05)
+        dh = randn(g, 40, 344, dtype=dt)
+        mean, rstd, gamma = torch.zeros(40, 1, device="cuda"), torch.ones(40, 1, device="cuda"), randn(g, 512, dtype=dt)
+        odd, odd_w = randn(g, 70, 301), randn(g, 2 * 33, 301)
+
+        def step():
+            h, pre = ops.gated_linear(x, w, "silu", save_pre=True)
+            return (h, *ops.gated_linear_backward(dh, x, w, pre, "silu"), ops.dropout_add(x, x, 0.3, (seed, 5)), ops.gated_linear(odd, odd_w, "gelu"),
+                    *ops.native_layer_norm_backward(x, x, [512], mean, rstd, gamma, gamma, [True] * 3))
+        return step
+
+    steps = [work(71), work(72)]
+    alone = [[t.clone() for t in s()] for s in steps]
+    torch.cuda.synchronize()
+    start, wrong, ended = threading.Barrier(2), [], []
+
+    def thread(i):
+        start.wait(60)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for n in range(100):
+                if not all(torch.equal(a, b) for a, b in zip(alone[i], steps[i]())):
+                    wrong.append((i, n))
+        ended.append(i)
+
+    threads = [threading.Thread(target=thread, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert sorted(ended) == [0, 1] and not wrong
