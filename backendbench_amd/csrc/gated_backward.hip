@@ -5,7 +5,10 @@
 // products do the rest.  dpre^T is written out (another 2 M F elements) because the product kernels run 25 % faster on a
 // K-contiguous left operand than on a transposed one: [22016, 4096] x [4096, 4096] takes 585 us from dpre as it is and 473
 // from its transpose, which costs 28 us to write.  dpre is rounded to the inputs' type: it is the operand of two matrix
-// products, whose matrix instructions take that type; everything before it is fp32 and the products accumulate in fp32.
+// products, whose matrix instructions take that type; everything before it is fp32 and the products accumulate in fp32.  A second
+// operand for what the rounding leaves out would double both products, 1.0 of the 1.1 ms at [4096, 4096] x 2 * 11008; without it the
+// error against 64 bits is 0.0023 of the result's norm in bf16, 0.0017 of it from rounding the result alone.  In f16 the rounding
+// bounds the range too: beyond 65504 dpre becomes infinite (a loss scale's overflow), in its row of dx and its row of dW alone.
 #include "gated.h"
 #include "elementwise.h"
 

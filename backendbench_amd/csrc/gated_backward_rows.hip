@@ -102,8 +102,9 @@ __global__ __launch_bounds__(64 * kGbrWaves, 2) void gated_backward_rows_kernel(
         w[2 * i + 1].load(W + (g.F + f) * g.w_rs + col);
       }
     }
-    // dpre.  In 16 bits the pair (gate's, up's) rounded to the type, as the matrix instructions of more rows take it: two
-    // terms to an operation, a third of the operations.
+    // dpre.  In 16 bits the pair (gate's, up's) rounded to the type, as the matrix instructions of more rows have to take it: one
+    // definition whatever the number of rows (in f16 with its range: infinite beyond 65504), and two terms to an operation, a third
+    // of the operations.
     A dgate[R], dup[R];
     uint32_t d2[R];
 #pragma unroll

@@ -200,7 +200,9 @@ def gated_linear_backward(grad_out, input, weight, pre, activation="silu", outpu
     """Gradients of gated_linear -> (grad_input, grad_weight), None where output_mask is False.
 
     pre: the pre-activations gated_linear(..., save_pre=True) returned.  The gradient of pre is computed in fp32 and
-    rounded once to the input's dtype: it is the operand of the two matrix products, which accumulate in fp32."""
+    rounded once to the input's dtype: it is the operand of the two matrix products, which accumulate in fp32.  In f16
+    that is also a bound on its range: a gradient of pre beyond 65504 becomes infinite, and with it its row of grad_input and its
+    row of grad_weight - nothing else - which is what a loss scale's check for infinities looks for."""
     _check_gated(input, weight, activation)
     F = weight.shape[0] // 2
     lead = list(input.shape[:-1])

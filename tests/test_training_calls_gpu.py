@@ -278,3 +278,19 @@ def test_operators_on_two_threads_at_once():
     for t in threads:
         t.join()
     assert sorted(ended) == [0, 1] and not wrong
+
+
+@pytest.mark.parametrize("M", [5, 16, 40, 300])
+def test_gated_linear_backward_f16_overflow_stays_in_its_row(M):
+    """f16: a gradient of pre beyond 65504 is infinite in its row of grad_input and its row of grad_weight and reaches nothing else."""
+    K, F, m0, f0 = 264, 136, 3, 77
+    g = generator(M)
+    x, w = randn(g, M, K, dtype=torch.float16), randn(g, 2 * F, K, dtype=torch.float16, scale=0.06)
+    pre, dh = randn(g, M, 2 * F, dtype=torch.float16), randn(g, M, F, dtype=torch.float16)
+    clean = ops.gated_linear_backward(dh, x, w, pre)
+    dh[m0, f0], pre[m0, f0], pre[m0, F + f0] = 60000.0, 3.0, 50.0  # d gate 3.3e6, d up 1.7e5
+    dx, dw = ops.gated_linear_backward(dh, x, w, pre)
+    rows, features = torch.ones(M, dtype=torch.bool, device="cuda"), torch.ones(2 * F, dtype=torch.bool, device="cuda")
+    rows[m0], features[f0], features[F + f0] = False, False, False
+    assert torch.equal(dx[rows], clean[0][rows]) and torch.equal(dw[features], clean[1][features])
+    assert not dx[m0].isfinite().any() and not dw[~features].isfinite().any()
