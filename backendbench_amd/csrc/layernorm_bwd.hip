@@ -19,9 +19,12 @@ constexpr int kLbMaxGroups = 256;  // row groups that leave a partial dw / db ea
 // The tile kernel: blocks of 1024 threads, GL lanes per row, EL = NV x V elements per lane.  One block per CU (at most 256
 // partials of dw / db, which the finish pass reads back from the last-level cache); sixteen waves of it, each with the
 // next row's loads in flight while it reduces the current one, keep 64 KB per CU outstanding.  x and dy stay in the
-// registers as loaded and are widened again after the two sums have met: 32 fp32 accumulators, two rows of raw vectors
-// and the weights fit the 128 registers that sixteen waves leave.  Rows of more than one wave meet in LDS, one barrier
-// per row (the slots alternate).
+// registers as loaded and are widened again after the two sums have met.  Sixteen waves leave 128 registers: a slab takes 40 - 89 of
+// them, two slabs of 32 fp32 accumulators, two rows of raw vectors and 16-bit weights 120 - 128 (one to four spilled to scratch
+// memory where N is no multiple of V).  fp32 weights beside 16-bit rows are too many: 6 registers spilled on 128 - 512 lanes, 16 on
+// 64, 8 - 22 where N is no multiple of V, 0 and 2 on 1024; the four slabs of fp32 rows spill 7 or 8.  The kernel alone, [10738,
+// 5056] bf16: 69 us with bf16 weights, 75 with fp32 ones, and 88 for 5053 columns, whose rows start off the vectors.
+// Rows of more than one wave meet in LDS, one barrier per row (the slots alternate).
 constexpr int kLbTile = 1024;
 // Columns of one gradient in a partial: padded so that every partial starts on a 16-byte boundary.
 __host__ __device__ constexpr int64_t lb_ld(int64_t N) { return (N + 3) / 4 * 4; }
