@@ -145,7 +145,7 @@ def gated_linear(input, weight, activation="silu", save_pre=False):
 def _rows_of(t):
     """`t` [R, K] itself when its rows are unit-stride and do not overlap, else a dense copy; one row K apart from the next
     (a tensor's own stride along a dimension of 1 says nothing: a column's transpose has 1)."""
-    if t.shape[0] == 1:
+    if t.shape[0] == 1 and t.stride() != (t.shape[1], 1):
         return dense(t).as_strided((1, t.shape[1]), (t.shape[1], 1))
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else dense(t)
 
@@ -259,8 +259,8 @@ def dropout_add(input, residual, p, rng):
     rng: (seed, offset), two Python integers or an int64 tensor of two.  An int64 tensor on the GPU is read by the
     kernel, so a captured graph draws anew once the program has advanced it.  Element i of input (in row-major order,
     whatever its strides) takes the i % 8-th 16 bits of Philox-4x32-10 at counter offset + i // 8 under key seed and is
-    dropped when they are below t = round(p * 65536), halves to the even neighbour; what is kept is scaled by 65536 / (65536 - t), which makes the
-    expectation exact for the p that 16 bits can hold.  Advance the offset by dropout_counters(input.numel())."""
+    dropped when they are below t = round(p * 65536), halves to the even neighbour; what is kept is scaled by
+    65536 / (65536 - t), which makes the expectation exact for the p that 16 bits can hold.  Advance the offset by dropout_counters(input.numel())."""
     _check_dropout(input, p, rng)
     if residual is not None and (residual.shape != input.shape or residual.dtype != input.dtype):
         raise RuntimeError(f"Expected residual of the input's shape and dtype, {list(input.shape)} {input.dtype}, but got "

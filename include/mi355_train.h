@@ -54,9 +54,9 @@ int mi355_pad_rows(const void* src, int64_t src_rs, int64_t R, int64_t C, void* 
 int mi355_gated_act(const void* pre, void* h, int dtype, int64_t M, int64_t F, int act, void* stream);
 
 /* The gated projection's gradients: dpre = [dh * up * act'(gate) | dh * act(gate)] with gate = pre[m][f], up = pre[m][F + f], rounded once to
- * `dtype` (f32, f16, bf16, f64), then dx [M][K] = dpre W and dweight [2F][K] = dpre^T x, accumulated in fp32 (fp64).  (f16: dpre beyond 65504 becomes
- * infinite, and with it its row of dx and of dweight.)  dh
- * [M][F], pre [M][2F], dx and dweight are dense; x and weight have rows x_rs and w_rs apart (one row of x: any x_rs).  dx or dweight may be NULL.
+ * `dtype` (f32, f16, bf16, f64), then dx [M][K] = dpre W and dweight [2F][K] = dpre^T x, accumulated in fp32 (fp64).
+ * (f16: dpre beyond 65504 becomes infinite, and with it its row of dx and of dweight.)  dh [M][F], pre [M][2F], dx and
+ * dweight are dense; x and weight have rows x_rs and w_rs apart (one row of x: any x_rs).  dx or dweight may be NULL.
  * The workspace (16-byte aligned, contents undefined before and after; not shared by calls that may overlap in time)
  * holds dpre and the products' scratch, or partial sums of dx: mi355_gated_linear_backward_workspace_bytes() always suffices. */
 int64_t mi355_gated_linear_backward_workspace_bytes(int64_t M, int64_t F, int64_t K, int dtype);
